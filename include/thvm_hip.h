@@ -136,8 +136,65 @@ void  thvm_hip_graph_destroy(void *graph);
 #define THVM_HIP_ENOTREADY (-2)
 #define THVM_HIP_ESCRATCH (-3)
 #define THVM_HIP_ENOSCRATCH (-4)
+#define THVM_HIP_ENOMEM (-5)
+#define THVM_HIP_EDEVICE (-6)
 int  thvm_hip_dispatch_uop_kernel_noalloc(u32 out_buf, const u32 *leaf_bufs, u32 n_leaves,
                                           const UOpKernel *kernel);
+
+/* Operators of a residual feed-forward block and of its training. No
+ * counterpart in the engine: a caller that builds such a block calls them
+ * between its dispatches, in the same order of work and on the same buffers.
+ *
+ * Buffers are ids, tensors in them dense and row-major from the buffer's
+ * start; id 0 is an absent operand where one may be. `dtype` (DTYPE_F32 or
+ * DTYPE_F16) is that of every tensor not named f32 here. All sums, statistics
+ * and products' sums are in 32 bits or more and an output is rounded once, to
+ * the nearest. Results are the same bits in every run. An operand may name
+ * the same buffer as an output only where it says so. Sizes of 0 are empty
+ * tensors, and their sums 0. The calls do not wait; workspaces come from the
+ * pool and stay for the next call. Returns THVM_HIP_OK, or:
+ *   THVM_HIP_EINVAL   not initialised, or arguments that cannot be (the reason
+ *                     goes to stderr); nothing is launched
+ *   THVM_HIP_ENOMEM   no memory for the workspace; nothing is launched
+ *   THVM_HIP_EDEVICE  a launch failed; outputs are undefined */
+#define THVM_HIP_ACT_NONE 0
+#define THVM_HIP_ACT_RELU 1
+#define THVM_HIP_ACT_GELU 2       /* z (1 + erf(z / sqrt 2)) / 2 */
+#define THVM_HIP_ACT_GELU_TANH 3  /* its tanh form */
+#define THVM_HIP_ACT_SILU 4       /* z / (1 + exp -z) */
+/* Layer norm of the rows of x [rows][cols]: y = (x - mean) * rstd * gamma +
+ * beta, rstd = 1 / sqrt(variance + eps). gamma and beta [cols] may be absent
+ * (1 and 0); mean and rstd [rows] f32 are kept where given. y may be x. */
+int  thvm_hip_layer_norm(u32 y, u32 mean, u32 rstd, u32 x, u32 gamma, u32 beta, u32 rows, u32 cols, f32 eps, u32 dtype);
+/* Its gradient from dy, x and the kept mean and rstd: dx [rows][cols], with
+ * `add` (0: nothing) added, the gradient that reaches x past the
+ * normalisation; dgamma and dbeta [cols]. Any of the three may be absent. dx
+ * may be dy, x or add. */
+int  thvm_hip_layer_norm_grad(u32 dx, u32 dgamma, u32 dbeta, u32 dy, u32 x, u32 mean, u32 rstd, u32 gamma, u32 add,
+                              u32 rows, u32 cols, u32 dtype);
+/* A linear layer y = act(z) + res, z = x W + bias: x [m][k], W [k][n], bias
+ * [n], res, z and y [m][n]. bias and res may be absent; z is kept where
+ * given, for the gradient. y may be res. 32-bit products are as exact as
+ * 32-bit sums of 32-bit products, infinities and NaN included. */
+int  thvm_hip_linear(u32 y, u32 z, u32 x, u32 w, u32 bias, u32 res, u32 act, u32 m, u32 k, u32 n, u32 dtype);
+/* Its gradient from dy and the kept z (not read without an activation): with
+ * dz = dy act'(z), dx = dz W^T, dw = x^T dz, db = the column sums of dz. That
+ * of res is dy itself. Any of the three may be absent, x without dw and w
+ * without dx. Of DTYPE_F16, the products take dz rounded to 16 bits. */
+int  thvm_hip_linear_grad(u32 dx, u32 dw, u32 db, u32 dy, u32 z, u32 x, u32 w, u32 act, u32 m, u32 k, u32 n, u32 dtype);
+/* One step of an optimiser whose update is orthogonalised, on `count`
+ * matrices [rows][cols] of one shape, each with its gradient and its momentum
+ * (f32), in place:
+ *   m = beta m + g;  u = nesterov ? g + beta m : m;  X = u / (|u| + 1e-7)
+ *   `steps` times:  A = X X^T, X = 3.4445 X + (-4.7750 A + 2.0315 A A) X
+ *   param = (1 - lr weight_decay) param - lr scale X
+ * |u| the Frobenius norm; the products run on the shorter side (X is u^T
+ * where rows > cols). After 5 steps X's singular values lie between 0.68 and
+ * 1.21 but for those that were under 1e-3 of |u|. `scale` is the caller's
+ * choice for the shape, such as sqrt(max(1, rows / cols)). Of DTYPE_F16, X,
+ * A and -4.7750 A + 2.0315 A A are rounded to 16 bits between products. */
+int  thvm_hip_muon_step(const u32 *param, const u32 *grad, const u32 *m, u32 count, u32 rows, u32 cols, f32 lr, f32 scale,
+                        f32 weight_decay, f32 beta, u32 nesterov, u32 steps, u32 dtype);
 
 /* Counters, for tests and the engine-driven timing (no counterpart in the
  * reference): out[0..15] = dispatches, matrix-core dispatches, compiled

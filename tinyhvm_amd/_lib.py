@@ -48,6 +48,11 @@ def lib():
                                   u32, u32]),
         "thvm_hip_op_reduce": (None, [u32, u32, u32, u32, u32, u32, u32, u32]),
         "thvm_hip_adam_step": (None, [u32, u32, u32, u32, f32, f32, f32, f32, f32, f32, u32]),
+        "thvm_hip_layer_norm": (C.c_int, [u32] * 8 + [f32, u32]),
+        "thvm_hip_layer_norm_grad": (C.c_int, [u32] * 12),
+        "thvm_hip_linear": (C.c_int, [u32] * 11),
+        "thvm_hip_linear_grad": (C.c_int, [u32] * 12),
+        "thvm_hip_muon_step": (C.c_int, [PU32, PU32, PU32, u32, u32, u32, f32, f32, f32, f32, u32, u32, u32]),
         "thvm_hip_graph_begin": (C.c_int, []),
         "thvm_hip_graph_end": (vp, []),
         "thvm_hip_graph_launch": (C.c_int, [vp]),
@@ -118,7 +123,8 @@ EXPORTED = ["hip_backend"] + [
     "thvm_hip_buf_incref", "thvm_hip_buf_decref", "thvm_hip_buf_write", "thvm_hip_buf_read",
     "thvm_hip_buf_read_nosync", "thvm_hip_dispatch_uop_kernel", "thvm_hip_dispatch_kernel_rs",
     "thvm_hip_contiguify", "thvm_hip_op_unary", "thvm_hip_op_binary", "thvm_hip_op_mm",
-    "thvm_hip_op_reduce", "thvm_hip_adam_step", "thvm_hip_graph_begin", "thvm_hip_graph_end",
+    "thvm_hip_op_reduce", "thvm_hip_adam_step", "thvm_hip_layer_norm", "thvm_hip_layer_norm_grad",
+    "thvm_hip_linear", "thvm_hip_linear_grad", "thvm_hip_muon_step", "thvm_hip_graph_begin", "thvm_hip_graph_end",
     "thvm_hip_graph_launch", "thvm_hip_graph_destroy", "thvm_hip_buf_copy", "thvm_hip_pool_reset",
     "thvm_hip_pool_set_persistent", "thvm_hip_profile_report", "thvm_hip_profile_reset",
     "thvm_hip_synchronize", "thvm_hip_counters", "thvm_hip_dispatch_uop_kernel_noalloc", "thvm_hip_stream", "thvm_hip_buf_device_ptr", "thvm_hip_backend",

@@ -1,8 +1,7 @@
 """Builds the HIP backend library in-tree.
 
-  1. hipcc --genco for gfx950: the precompiled kernels (static_kernels.hip and
-     the dense kernels) -> one code object;
-  2. the code object is embedded into a C file as a byte array;
+  1. hipcc --genco for gfx950: each file of precompiled kernels -> a code object;
+  2. the code objects are embedded into C files as byte arrays;
   3. hipcc -c: noalloc.hip (a device array and its address lookup);
   4. gcc (plain C, HIP runtime C API) -> tinyhvm_amd/libthvm_hip.so.
 
@@ -11,6 +10,7 @@ Run: python -m tinyhvm_amd.build
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -24,8 +24,10 @@ LIB_PATH = os.path.join(HERE, LIB_NAME)
 # no FP contraction: a*b+c stays two rounded operations, as in the x86 engine
 HIP_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off",
              "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-HOST_SOURCES = ["backend.c", "pool.c", "kgen.c", "rtc.c", "affine.c", "dense.c", "window.c", "chain.c", "replay.c"]
-KERNEL_SOURCES = ["static_kernels.hip"]
+HOST_SOURCES = ["backend.c", "pool.c", "kgen.c", "rtc.c", "affine.c", "dense.c", "window.c", "chain.c", "block.c", "replay.c"]
+KERNEL_SOURCES = ["static_kernels.hip", "norm_kernels.hip", "gemm_kernels.hip"]
+# operators the engine has no counterpart of, whose roundings no one else repeats
+CONTRACTED = {"norm_kernels.hip", "gemm_kernels.hip"}
 # host + device code built by hipcc into an object: the static device workspace
 # of the no-allocation entry point, whose address hipGetSymbolAddress looks up
 HIP_OBJECTS = ["noalloc.hip"]
@@ -39,23 +41,29 @@ def _run(cmd):
     return r
 
 
-def build_kernels():
-    os.makedirs(BUILD, exist_ok=True)
-    srcs = [os.path.join(CSRC, s) for s in KERNEL_SOURCES if os.path.exists(os.path.join(CSRC, s))]
-    co = os.path.join(BUILD, "static_kernels.hsaco")
-    _run([os.path.join(ROCM, "bin", "hipcc"), "--genco"] + HIP_FLAGS +
-         ["-I" + INC, "-I" + CSRC] + srcs + ["-o", co])
+def _embed(source):
+    """C file that holds the code object of one kernel source as
+    thvm_<name>_co."""
+    name = os.path.splitext(source)[0]
+    co = os.path.join(BUILD, name + ".hsaco")
+    flags = ["-ffp-contract=fast" if f == "-ffp-contract=off" and source in CONTRACTED else f for f in HIP_FLAGS]
+    _run([os.path.join(ROCM, "bin", "hipcc"), "--genco"] + flags +
+         ["-I" + INC, "-I" + CSRC, os.path.join(CSRC, source), "-o", co])
     data = open(co, "rb").read()
-    blob = os.path.join(BUILD, "static_kernels_blob.c")
+    blob = os.path.join(BUILD, name + "_blob.c")
     with open(blob, "w") as f:
-        f.write("/* generated by tinyhvm_amd/build.py from the static kernel code object */\n")
-        f.write("const unsigned long thvm_static_kernels_co_len = %dUL;\n" % len(data))
-        f.write("__attribute__((aligned(4096))) const unsigned char thvm_static_kernels_co[%d] = {\n"
-                % len(data))
+        f.write("/* generated by tinyhvm_amd/build.py from a kernel code object */\n")
+        f.write("__attribute__((aligned(4096))) const unsigned char thvm_%s_co[%d] = {\n" % (name, len(data)))
         for i in range(0, len(data), 24):
             f.write("  " + ",".join(str(b) for b in data[i:i + 24]) + ",\n")
         f.write("};\n")
     return blob
+
+
+def build_kernels():
+    os.makedirs(BUILD, exist_ok=True)
+    with ThreadPoolExecutor(len(KERNEL_SOURCES)) as pool:
+        return list(pool.map(_embed, KERNEL_SOURCES))
 
 
 def build_hip_objects():
@@ -70,13 +78,13 @@ def build_hip_objects():
 
 
 def build_library():
-    blob = build_kernels()
+    blobs = build_kernels()
     objs = build_hip_objects()
     srcs = [os.path.join(CSRC, s) for s in HOST_SOURCES if os.path.exists(os.path.join(CSRC, s))]
     tmp = LIB_PATH + ".tmp"
     _run(["gcc", "-std=gnu11", "-O2", "-fPIC", "-shared", "-Wall", "-Wno-unused-function",
           "-D__HIP_PLATFORM_AMD__", "-I" + os.path.join(ROCM, "include"), "-I" + INC, "-I" + CSRC]
-         + srcs + [blob] + objs + ["-L" + os.path.join(ROCM, "lib"), "-lamdhip64", "-lhiprtc",
+         + srcs + blobs + objs + ["-L" + os.path.join(ROCM, "lib"), "-lamdhip64", "-lhiprtc",
                                    "-lstdc++", "-lpthread", "-lm", "-Wl,-rpath," + os.path.join(ROCM, "lib"),
                                    "-o", tmp])
     os.replace(tmp, LIB_PATH)

@@ -66,6 +66,13 @@ static void copyq_guard(u32 id) {
     if (CQ.b.n && id && copyq_uses(id)) copyq_flush();
 }
 
+/* A buffer that an operator of block.c takes: queued copies of it and its
+ * pending host write go ahead of the operator's work. */
+void hipb_operand(u32 id) {
+    copyq_guard(id);
+    pool_sync_device(id);
+}
+
 static void copyq_guard_dispatch(u32 out, const u32 *leaves, u32 n) {
     if (!CQ.b.n) return;
     copyq_guard(out);
@@ -1371,6 +1378,7 @@ static void hb_shutdown(void) {
     graphs_release_all();
     dense_shutdown();
     window_shutdown();
+    block_shutdown();
     hb_release();
     upload_release();
     rtc_shutdown();

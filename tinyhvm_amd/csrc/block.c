@@ -1,0 +1,533 @@
+/*
+ * block.c - the operators of a residual feed-forward block and of its
+ * training: layer norm, a linear layer with bias, activation and residual,
+ * their gradients, and an orthogonalised optimiser step. Entry points of
+ * thvm_hip.h with no counterpart in the engine; kernels in norm_kernels.hip
+ * and gemm_kernels.hip. They take buffer ids like the Backend slots, put
+ * their work on the backend's stream, and never wait on the host.
+ */
+#include <math.h>
+#include <string.h>
+
+#include "hipb.h"
+#include "thvm_hip.h"
+#include "block_args.h"
+
+static Scratch block_ws;
+
+void block_shutdown(void) { scratch_release(&block_ws); }
+
+/* ---- arguments ---- */
+
+static int refuse(const char *op, const char *why) {
+    fprintf(stderr, "tinyhvm-hip: %s: %s\n", op, why);
+    return THVM_HIP_EINVAL;
+}
+
+typedef struct { u32 id; u64 bytes; int out; } Operand;
+
+/* Every named buffer exists and holds its tensor, and no output is also
+ * another operand. `same` lists pairs (output, input) that may be one buffer. */
+static int operands_ok(const char *op, const Operand *o, u32 n, const u32 (*same)[2], u32 n_same) {
+    for (u32 i = 0; i < n; i++) {
+        if (!o[i].id) continue;
+        if (!pool_get(o[i].id)) { refuse(op, "an unknown buffer"); return 0; }
+        if (pool_bytes(o[i].id) < o[i].bytes) { refuse(op, "a buffer shorter than its tensor"); return 0; }
+        for (u32 j = 0; j < n; j++) {
+            if (j == i || o[j].id != o[i].id || !o[i].out) continue;
+            int ok = 0;
+            for (u32 s = 0; s < n_same; s++) ok |= same[s][0] == i && same[s][1] == j;
+            for (u32 s = 0; s < n_same; s++) ok |= same[s][0] == j && same[s][1] == i;
+            if (!ok) { refuse(op, "an output is also another operand"); return 0; }
+        }
+    }
+    return 1;
+}
+
+/* The operands' pending copies and host writes go ahead of the work. */
+static void operands_ready(const Operand *o, u32 n) {
+    for (u32 i = 0; i < n; i++)
+        if (o[i].id) hipb_operand(o[i].id);
+}
+
+static void operands_written(const Operand *o, u32 n) {
+    for (u32 i = 0; i < n; i++)
+        if (o[i].id && o[i].out) pool_mark_device_write(o[i].id);
+}
+
+static u64 addr(u32 id) { return id ? (u64)(uintptr_t)pool_ptr(id) : 0; }
+
+static int dtype_ok(u32 dtype) { return dtype == DTYPE_F32 || dtype == DTYPE_F16; }
+static u64 esize(u32 dtype) { return dtype == DTYPE_F16 ? 2 : 4; }
+static const char *tname(u32 dtype) { return dtype == DTYPE_F16 ? "f16" : "f32"; }
+
+static u64 div_up(u64 a, u64 b) { return (a + b - 1) / b; }
+static u64 round_up(u64 a, u64 b) { return div_up(a, b) * b; }
+
+/* Work on the stream, in order; the first failure ends it. */
+static int launch(const char *name, u64 gx, u32 gy, u32 gz, u32 bx, void **params) {
+    if (!gx || !gy || !gz) return THVM_HIP_OK;
+    if (gx * bx >= (1ull << 32) || gy > 65535 || gz > 65535) {
+        fprintf(stderr, "tinyhvm-hip: %s: the grid exceeds the launch limit\n", name);
+        return THVM_HIP_EINVAL;
+    }
+    hipFunction_t fn = rtc_static_fn(name);
+    if (!fn || !hipb_launch(fn, (u32)gx, gy, gz, bx, params)) return THVM_HIP_EDEVICE;
+    return THVM_HIP_OK;
+}
+static int launch1(const char *name, u64 gx, u32 gy, u32 gz, u32 bx, void *args) {
+    void *params[] = {args};
+    return launch(name, gx, gy, gz, bx, params);
+}
+
+/* A workspace's parts, one after another. */
+typedef struct { u64 bytes; u64 base; } Carve;
+static u64 carve(Carve *c, u64 bytes) {
+    u64 at = c->base + c->bytes;
+    c->bytes += round_up(bytes, 1024);
+    return at;
+}
+static int carve_reserve(Carve *c) {
+    void *p = scratch_reserve(&block_ws, c->bytes ? c->bytes : 1024);
+    if (!p) return 0;
+    c->base = (u64)(uintptr_t)p;
+    c->bytes = 0;
+    return 1;
+}
+
+/* ---- layer norm ---- */
+
+/* Lanes a row (64 a wave of its own, else a workgroup) and vectors a lane. */
+static int ln_shape(u32 rows, u32 cols, u32 dtype, u32 *g, u32 *nv) {
+    const u64 vecs = div_up(cols, 16 / esize(dtype));
+    *g = vecs <= 256 && (rows >= 1024 || vecs <= 64) ? 64 : vecs <= 1024 && rows >= 256 ? 256 : 1024;
+    if (*g == 1024 && vecs <= 256) *g = 256;
+    if (*g == 256 && vecs > 2048) *g = 1024;
+    for (*nv = 1; *nv * *g < vecs; *nv *= 2) {}
+    return *nv <= (*g == 1024 ? 4u : 8u);
+}
+
+int thvm_hip_layer_norm(u32 y, u32 mean, u32 rstd, u32 x, u32 gamma, u32 beta, u32 rows, u32 cols, f32 eps, u32 dtype) {
+    if (!hipb.initialized) return THVM_HIP_EINVAL;
+    const char *op = "layer_norm";
+    if (!dtype_ok(dtype)) return refuse(op, "the type is neither f32 nor f16");
+    if (!y || !x) return refuse(op, "no input or no output");
+    const u64 n = (u64)rows * cols * esize(dtype), v = cols * esize(dtype), st = rows * 4ull;
+    const Operand o[] = {{y, n, 1}, {mean, st, 1}, {rstd, st, 1}, {x, n, 0}, {gamma, v, 0}, {beta, v, 0}};
+    const u32 same[][2] = {{0, 3}};
+    if (!operands_ok(op, o, 6, same, 1)) return THVM_HIP_EINVAL;
+    if (!rows || !cols) return THVM_HIP_OK;
+    operands_ready(o, 6);
+    u32 g, nv;
+    char name[48];
+    const int fits = ln_shape(rows, cols, dtype, &g, &nv);
+    if (fits) snprintf(name, sizeof name, "thvm_ln_%s_%u_%u", tname(dtype), g, nv);
+    else snprintf(name, sizeof name, "thvm_ln_%s_long", tname(dtype)), g = 1024;
+    int rc = THVM_HIP_OK;
+    /* a launch holds fewer than 2^32 lanes */
+    for (u32 r0 = 0, step = (1u << 31) / g; r0 < rows && !rc; r0 += step) {
+        const u32 nr = rows - r0 < step ? rows - r0 : step;
+        const u64 off = (u64)r0 * v;
+        LnArgs a = {addr(x) + off, addr(gamma), addr(beta), addr(y) + off, mean ? addr(mean) + r0 * 4ull : 0,
+                    rstd ? addr(rstd) + r0 * 4ull : 0, nr, cols, eps, 0};
+        rc = launch1(name, g < 256 ? div_up(nr, 256 / g) : nr, 1, 1, g < 256 ? 256 : g, &a);
+    }
+    operands_written(o, 6);
+    return rc;
+}
+
+int thvm_hip_layer_norm_grad(u32 dx, u32 dgamma, u32 dbeta, u32 dy, u32 x, u32 mean, u32 rstd, u32 gamma, u32 add,
+                             u32 rows, u32 cols, u32 dtype) {
+    if (!hipb.initialized) return THVM_HIP_EINVAL;
+    const char *op = "layer_norm_grad";
+    if (!dtype_ok(dtype)) return refuse(op, "the type is neither f32 nor f16");
+    if (!dy || !x || !mean || !rstd) return refuse(op, "no gradient, input or statistics");
+    if (!dx && !dgamma && !dbeta) return refuse(op, "no output");
+    const u64 n = (u64)rows * cols * esize(dtype), v = cols * esize(dtype), st = rows * 4ull;
+    const Operand o[] = {{dx, n, 1}, {dgamma, v, 1}, {dbeta, v, 1}, {dy, n, 0}, {x, n, 0},
+                         {mean, st, 0}, {rstd, st, 0}, {gamma, v, 0}, {add, n, 0}};
+    const u32 same[][2] = {{0, 3}, {0, 4}, {0, 8}};
+    if (!operands_ok(op, o, 9, same, 3)) return THVM_HIP_EINVAL;
+    if (!cols) return THVM_HIP_OK;
+    const u64 vecs = div_up(cols, 16 / esize(dtype));
+    const int wgrad = dgamma || dbeta, half = dtype == DTYPE_F16;
+    /* the kernels' shapes (norm_kernels.hip) */
+    u32 g = 0, nv = 0;
+    if (vecs <= (half ? 128 : 256)) for (g = 64, nv = 1; nv * g < vecs;) nv *= 2;
+    else if (vecs <= (half ? 512 : 1024)) for (g = 256, nv = half ? 1 : 2; nv * g < vecs;) nv *= 2;
+    else if (vecs <= (half ? 2048 : 4096)) for (g = 512, nv = half ? 2 : 4; nv * g < vecs;) nv *= 2;
+    u32 parts;
+    if (g) {
+        const u32 per = g < 256 ? 256 / g : 1, full = hipb.n_cu * (g == 512 ? 1 : 2);
+        parts = (u32)(div_up(rows, per) < full ? div_up(rows, per) : full);
+    } else parts = (u32)(div_up(rows, 64) < 256 ? div_up(rows, 64) : 256);
+    Carve c = {0, 0};
+    carve(&c, wgrad ? 8ull * parts * cols : 0);
+    if (!carve_reserve(&c)) return THVM_HIP_ENOMEM;
+    operands_ready(o, 9);
+    LnGradArgs a = {addr(dy), addr(x), addr(mean), addr(rstd), addr(gamma), addr(add), addr(dx), addr(dgamma), addr(dbeta),
+                    wgrad ? carve(&c, 0) : 0, rows, cols, parts, 0};
+    char name[48];
+    int rc = THVM_HIP_OK;
+    if (g) {
+        snprintf(name, sizeof name, "thvm_lnb_%s_%u_%u", tname(dtype), g, nv);
+        rc = launch1(name, parts, 1, 1, g < 256 ? 256 : g, &a);
+    } else {
+        if (wgrad) {
+            snprintf(name, sizeof name, "thvm_lnb_%s_part", tname(dtype));
+            rc = launch1(name, div_up(cols, 256), parts, 1, 256, &a);
+        }
+        snprintf(name, sizeof name, "thvm_lnb_%s_long", tname(dtype));
+        for (u32 r0 = 0, step = 1u << 21; dx && r0 < rows && !rc; r0 += step) {
+            const u64 off = (u64)r0 * v;
+            LnGradArgs b = a;
+            b.rows = rows - r0 < step ? rows - r0 : step;
+            b.dy += off; b.x += off; b.dx += off;
+            if (b.add) b.add += off;
+            b.mean += r0 * 4ull; b.rstd += r0 * 4ull;
+            rc = launch1(name, b.rows, 1, 1, 1024, &b);
+        }
+    }
+    if (wgrad && !rc) {
+        snprintf(name, sizeof name, "thvm_lnb_%s_cols", tname(dtype));
+        rc = launch1(name, div_up(2ull * cols, 64), 1, 1, 1024, &a);
+    }
+    operands_written(o, 9);
+    return rc;
+}
+
+/* ---- products ---- */
+
+/* A packed operand of `rows` rows by `k`, padded to whole tiles. */
+typedef struct { u32 Rp, KB; u64 p, e; } Packed;
+
+static u64 packed_bytes(const Packed *k, u32 dtype) { return (u64)k->Rp * k->KB * 32 * (dtype == DTYPE_F16 ? 1 : 2); }
+
+static Packed packed_of(u32 rows, u32 k, u32 tile) {
+    Packed p = {(u32)round_up(rows, tile), (u32)(round_up(k, 64) / 16), 0, 0};
+    return p;
+}
+
+static void packed_carve(Packed *p, Carve *c, u32 dtype) {
+    p->p = carve(c, packed_bytes(p, dtype));
+    p->e = carve(c, dtype == DTYPE_F32 ? p->Rp * 4ull : 0);
+}
+
+/* A product's tile and K splits: C [M][N] over K. */
+typedef struct { u32 tile, tm, tn, splits; } Plan;
+
+static Plan plan_of(u32 M, u32 N, u32 K, u32 dtype) {
+    static const u32 sizes[] = {256, 128, 64};
+    const u32 cu = hipb.n_cu ? hipb.n_cu : 256;
+    Plan p = {0, 0, 0, 1};
+    for (u32 i = 0; i < 3; i++) {
+        p.tile = sizes[i];
+        p.tm = (u32)div_up(M, p.tile);
+        p.tn = (u32)div_up(N, p.tile);
+        if ((u64)p.tm * p.tn >= cu * 3 / 4) break;
+    }
+    const u64 tiles = (u64)p.tm * p.tn, stages = round_up(K, 64) / (dtype == DTYPE_F16 ? 64 : 32);
+    while (tiles * p.splits * 2 <= cu * 2 && stages / (p.splits * 2) >= 4 && p.splits < 16) p.splits *= 2;
+    return p;
+}
+
+static u64 plan_part_bytes(const Plan *p, u32 M, u32 N) { return p->splits > 1 ? 4ull * p->splits * M * N : 0; }
+
+/* The product of two packed operands with its epilogue (a: out, z, bias, res, act). */
+static int product(const Plan *pl, const Packed *A, const Packed *B, u32 M, u32 N, u32 dtype, u64 part, GemmArgs a) {
+    char name[48];
+    a.A = A->p; a.B = B->p; a.ea = A->e; a.eb = B->e;
+    a.M = M; a.N = N; a.KB = A->KB;
+    a.tm = pl->tm; a.tn = pl->tn; a.splits = pl->splits; a.part = part;
+    snprintf(name, sizeof name, "thvm_gemm_%u_%s", pl->tile, tname(dtype));
+    int rc = launch1(name, (u64)pl->tm * pl->tn, pl->splits, 1, pl->tile == 256 ? 512 : 256, &a);
+    if (rc || pl->splits == 1) return rc;
+    snprintf(name, sizeof name, "thvm_gemm_join_%s", tname(dtype));
+    return launch1(name, div_up(div_up(N, 8) * M, 256), 1, 1, 256, &a);
+}
+
+/* Packing of a matrix [R][C] (times act'(z) where z is given): `rows` with
+ * its rows as rows, `cols` with its columns, either or both; and the partial
+ * column sums. Parts live in the workspace from `parts` on. */
+#define SIZE_COLS 512u
+#define SIZE_PARTS 64u
+static u64 pack_parts_bytes(u32 R, u32 C, u32 dtype) {
+    if (dtype == DTYPE_F16) return 4ull * div_up(R, 64) * C;
+    return 4ull * div_up(C, SIZE_COLS) * R + 2 * 4ull * SIZE_PARTS * C + 3072;
+}
+
+static int pack(u64 src, u64 z, u32 act, u32 R, u32 C, u32 dtype, const Packed *rows, const Packed *cols, u64 parts,
+                u64 sums_out) {
+    char name[48];
+    PackArgs a;
+    memset(&a, 0, sizeof a);
+    a.src = src; a.z = act ? z : 0; a.act = act; a.R = R; a.C = C;
+    int rc = THVM_HIP_OK;
+    u32 sum_parts = (u32)div_up(R, 64);
+    if (dtype == DTYPE_F32) {
+        Carve c = {0, parts};
+        a.rt = (u32)(div_up(div_up(R, SIZE_PARTS), 8) * 8);
+        if (a.rt < 32) a.rt = 32;
+        a.row_parts = (u32)div_up(C, SIZE_COLS);
+        a.col_parts = sum_parts = (u32)div_up(R, a.rt);
+        if (rows) a.row_part = carve(&c, 4ull * a.row_parts * R);
+        if (cols) a.col_part = carve(&c, 4ull * a.col_parts * C);
+        if (sums_out) a.sum_part = carve(&c, 4ull * a.col_parts * C);
+        snprintf(name, sizeof name, "thvm_pack_sizes_%s", tname(dtype));
+        rc = launch1(name, a.row_parts, a.col_parts, 1, 512, &a);
+    } else if (sums_out) a.sum_part = parts;
+    if (!rc && (rows || cols || dtype == DTYPE_F16)) {
+        PackArgs b = a;
+        if (dtype == DTYPE_F32) b.sum_part = 0;
+        u32 rmax = (u32)round_up(R, 64), cmax = (u32)round_up(C, 64);
+        if (rows) {
+            b.pn = rows->p; b.en = rows->e; b.Rn = rows->Rp; b.KBn = rows->KB;
+            if (rows->Rp > rmax) rmax = rows->Rp;
+        }
+        if (cols) {
+            b.pt = cols->p; b.et = cols->e; b.Ct = cols->Rp; b.KBt = cols->KB;
+            if (cols->Rp > cmax) cmax = cols->Rp;
+        }
+        b.ctiles = cmax / 64;
+        /* column sums are written once a row tile of the matrix itself */
+        snprintf(name, sizeof name, "thvm_pack_%s", tname(dtype));
+        rc = launch1(name, (u64)(rmax / 64) * b.ctiles, 1, 1, 256, &b);
+        if (dtype == DTYPE_F16) sum_parts = (u32)div_up(R, 64);
+    }
+    if (!rc && sums_out) {
+        void *params[] = {&a.sum_part, &sums_out, &C, &sum_parts};
+        snprintf(name, sizeof name, "thvm_sum_parts_%s", tname(dtype));
+        rc = launch(name, div_up(C, 64), 1, 1, 1024, params);
+    }
+    return rc;
+}
+
+/* Few rows: W is read as it lies (few_rows in gemm_kernels.hip). */
+static int few(u32 m, u32 k, u32 n, u32 dtype, GemmArgs a) {
+    const u32 cols = 16 * (u32)(16 / esize(dtype)), mr = m <= 1 ? 1 : m <= 4 ? 4 : 16;
+    const u64 strips = div_up(n, cols), blocks = div_up(m, mr), chunks = div_up(k ? k : 1, 128);
+    u64 splits = 512 / (strips * blocks);
+    if (splits < 1) splits = 1;
+    if (splits > chunks) splits = chunks;
+    if (splits > 64) splits = 64;
+    a.kper = (u32)(div_up(chunks, splits) * 128);
+    a.splits = (u32)div_up(k ? k : 1, a.kper);
+    a.M = m; a.N = n; a.K = k;
+    Carve c = {0, 0};
+    carve(&c, a.splits > 1 ? 4ull * a.splits * m * n : 0);
+    if (!carve_reserve(&c)) return THVM_HIP_ENOMEM;
+    a.part = carve(&c, 0);
+    char name[48];
+    snprintf(name, sizeof name, "thvm_few%u_%s", mr, tname(dtype));
+    int rc = launch1(name, strips, a.splits, (u32)blocks, 512, &a);
+    if (rc || a.splits == 1) return rc;
+    snprintf(name, sizeof name, "thvm_few_join_%s", tname(dtype));
+    return launch1(name, div_up(div_up(n, 8) * m, 256), 1, 1, 256, &a);
+}
+
+int thvm_hip_linear(u32 y, u32 z, u32 x, u32 w, u32 bias, u32 res, u32 act, u32 m, u32 k, u32 n, u32 dtype) {
+    if (!hipb.initialized) return THVM_HIP_EINVAL;
+    const char *op = "linear";
+    if (!dtype_ok(dtype)) return refuse(op, "the type is neither f32 nor f16");
+    if (act >= ACT_COUNT) return refuse(op, "an unknown activation");
+    if (!y || !x || !w) return refuse(op, "no input, weights or output");
+    const u64 es = esize(dtype), mn = (u64)m * n * es;
+    const Operand o[] = {{y, mn, 1}, {z, mn, 1}, {x, (u64)m * k * es, 0}, {w, (u64)k * n * es, 0}, {bias, n * es, 0}, {res, mn, 0}};
+    const u32 same[][2] = {{0, 5}};
+    if (!operands_ok(op, o, 6, same, 1)) return THVM_HIP_EINVAL;
+    if (!m || !n) return THVM_HIP_OK;
+    GemmArgs a;
+    memset(&a, 0, sizeof a);
+    a.out = addr(y); a.z = addr(z); a.bias = addr(bias); a.res = addr(res); a.act = act;
+    int rc;
+    if (m <= 16 || !k) {
+        operands_ready(o, 6);
+        a.A = addr(x); a.B = addr(w);
+        rc = few(m, k, n, dtype, a);
+    } else {
+        const Plan pl = plan_of(m, n, k, dtype);
+        Packed px = packed_of(m, k, pl.tile), pw = packed_of(n, k, pl.tile);
+        u64 parts = 0, part = 0;
+        Carve c = {0, 0};
+        for (int pass = 0; pass < 2; pass++) {
+            packed_carve(&px, &c, dtype);
+            packed_carve(&pw, &c, dtype);
+            u64 b = pack_parts_bytes(m, k, dtype), b2 = pack_parts_bytes(k, n, dtype);
+            parts = carve(&c, dtype == DTYPE_F32 ? (b > b2 ? b : b2) : 0);
+            part = carve(&c, plan_part_bytes(&pl, m, n));
+            if (!pass && !carve_reserve(&c)) return THVM_HIP_ENOMEM;
+        }
+        operands_ready(o, 6);
+        rc = pack(addr(x), 0, 0, m, k, dtype, &px, NULL, parts, 0);
+        if (!rc) rc = pack(addr(w), 0, 0, k, n, dtype, NULL, &pw, parts, 0);
+        if (!rc) rc = product(&pl, &px, &pw, m, n, dtype, part, a);
+    }
+    operands_written(o, 6);
+    return rc;
+}
+
+int thvm_hip_linear_grad(u32 dx, u32 dw, u32 db, u32 dy, u32 z, u32 x, u32 w, u32 act, u32 m, u32 k, u32 n, u32 dtype) {
+    if (!hipb.initialized) return THVM_HIP_EINVAL;
+    const char *op = "linear_grad";
+    if (!dtype_ok(dtype)) return refuse(op, "the type is neither f32 nor f16");
+    if (act >= ACT_COUNT) return refuse(op, "an unknown activation");
+    if (!dy || (act && !z) || (dx && !w) || (dw && !x)) return refuse(op, "no gradient, input or weights, or no values before the activation");
+    if (!dx && !dw && !db) return refuse(op, "no output");
+    const u64 es = esize(dtype), mn = (u64)m * n * es;
+    const Operand o[] = {{dx, (u64)m * k * es, 1}, {dw, (u64)k * n * es, 1}, {db, n * es, 1}, {dy, mn, 0},
+                         {act ? z : 0, mn, 0}, {dw ? x : 0, (u64)m * k * es, 0}, {dx ? w : 0, (u64)k * n * es, 0}};
+    if (!operands_ok(op, o, 7, NULL, 0)) return THVM_HIP_EINVAL;
+    /* an empty sum is 0: gradients over no rows or no outputs */
+    if (!k) dx = dw = 0;
+    if (!m) dx = 0;
+    if (!n) dw = db = 0;
+    if (!dx && !dw && !db) return THVM_HIP_OK;
+    const Plan px_ = plan_of(m, k, n, dtype), pw_ = plan_of(k, n, m, dtype);
+    Packed zr = packed_of(m, n, px_.tile), wr = packed_of(k, n, px_.tile);       /* dx = dz W^T */
+    Packed xc = packed_of(k, m, pw_.tile), zc = packed_of(n, m, pw_.tile);       /* dW = x^T dz */
+    u64 parts = 0, part = 0;
+    Carve c = {0, 0};
+    for (int pass = 0; pass < 2; pass++) {
+        if (dx) packed_carve(&zr, &c, dtype), packed_carve(&wr, &c, dtype);
+        if (dw) packed_carve(&xc, &c, dtype), packed_carve(&zc, &c, dtype);
+        u64 b = pack_parts_bytes(m, n, dtype), b2 = dtype == DTYPE_F32 ? pack_parts_bytes(k, n, dtype) : 0;
+        u64 b3 = dtype == DTYPE_F32 ? pack_parts_bytes(m, k, dtype) : 0;
+        if (b2 > b) b = b2;
+        if (b3 > b) b = b3;
+        parts = carve(&c, b);
+        u64 q = dx ? plan_part_bytes(&px_, m, k) : 0, q2 = dw ? plan_part_bytes(&pw_, k, n) : 0;
+        part = carve(&c, q > q2 ? q : q2);
+        if (!pass && !carve_reserve(&c)) return THVM_HIP_ENOMEM;
+    }
+    operands_ready(o, 7);
+    GemmArgs a;
+    memset(&a, 0, sizeof a);
+    int rc = pack(addr(dy), addr(z), act, m, n, dtype, dx ? &zr : NULL, dw ? &zc : NULL, parts, addr(db));
+    if (dx) {
+        if (!rc) rc = pack(addr(w), 0, 0, k, n, dtype, &wr, NULL, parts, 0);
+        a.out = addr(dx);
+        if (!rc) rc = product(&px_, &zr, &wr, m, k, dtype, part, a);
+    }
+    if (dw) {
+        if (!rc) rc = pack(addr(x), 0, 0, m, k, dtype, NULL, &xc, parts, 0);
+        a.out = addr(dw);
+        if (!rc) rc = product(&pw_, &xc, &zc, k, n, dtype, part, a);
+    }
+    operands_written(o, 7);
+    return rc;
+}
+
+/* ---- the orthogonalised step ---- */
+
+/* x -> a x + b x^3 + c x^5 on the singular values, the steepest such step at
+ * 0 that keeps [0, 1.2] within itself and ends near 1 */
+#define NS_A 3.4445
+#define NS_B (-4.7750)
+#define NS_C 2.0315
+/* X and A = X X^T are packed times 2^14, B = b A + c A^2 times 2^13: |X| and
+ * |A| stay under 1.5 and |B| under 2.9, so all of them stay under 2^16 */
+
+static int muon_chunk(const u32 *param, const u32 *grad, const u32 *m, u32 count, u32 rows, u32 cols, f32 keep, f32 step,
+                      f32 beta, int nesterov, u32 steps, u32 dtype, u32 tile) {
+    char name[48];
+    const int tall = rows > cols;
+    const u32 n = tall ? cols : rows, w = tall ? rows : cols;
+    const u32 np = (u32)round_up(n, tile), wp = (u32)round_up(w, tile);
+    const u64 pl = dtype == DTYPE_F16 ? 1 : 2, xb = round_up(2ull * pl * np * wp, 1024), ab = round_up(2ull * pl * np * np, 1024);
+    MuonArgs mu;
+    memset(&mu, 0, sizeof mu);
+    mu.numel = (u64)rows * cols;
+    mu.blocks = (u32)(div_up(mu.numel, 1024) < 1024 ? div_up(mu.numel, 1024) : 1024);
+    mu.nesterov = nesterov != 0;
+    mu.beta = beta;
+    /* a matrix's operands, `stride` bytes in all: X, X^T twice, A, B */
+    const u64 stride = 3 * xb + 2 * ab;
+    u64 ops = 0;
+    Carve c = {0, 0};
+    for (int pass = 0; pass < 2; pass++) {
+        ops = carve(&c, stride * count);
+        mu.sums = carve(&c, 8ull * mu.blocks * count);
+        if (!pass && !carve_reserve(&c)) return THVM_HIP_ENOMEM;
+    }
+    NsArgs a;
+    memset(&a, 0, sizeof a);
+    for (u32 i = 0; i < count; i++) {
+        a.param[i] = addr(param[i]);
+        mu.grad[i] = addr(grad[i]);
+        mu.m[i] = addr(m[i]);
+    }
+    snprintf(name, sizeof name, "thvm_muon_momentum_%s", tname(dtype));
+    int rc = launch1(name, mu.blocks, count, 1, 256, &mu);
+    if (rc) return rc;
+    PackArgs p;
+    memset(&p, 0, sizeof p);
+    const u64 X = ops, A = ops + 3 * xb, B = A + ab;
+    u64 xt = ops + xb, xt2 = ops + 2 * xb;
+    p.R = rows; p.C = cols; p.stride = stride;
+    p.pn = tall ? xt : X; p.Rn = tall ? wp : np; p.KBn = (tall ? np : wp) / 16;
+    p.pt = tall ? X : xt; p.Ct = tall ? np : wp; p.KBt = (tall ? wp : np) / 16;
+    p.ctiles = p.Ct / 64;
+    void *pp[] = {&p, &mu};
+    snprintf(name, sizeof name, "thvm_muon_pack_%s", tname(dtype));
+    rc = launch(name, (u64)(p.Rn / 64) * p.ctiles, count, 1, 256, pp);
+    snprintf(name, sizeof name, "thvm_ns_%u_%s", tile, tname(dtype));
+    const u32 tn = np / tile, tw = wp / tile, lanes = tile == 256 ? 512 : 256, half = tn * (tn + 1) / 2;
+    a.stride = stride; a.n = n; a.w = w; a.tall = (u32)tall; a.keep = keep; a.step = step;
+    for (u32 s = 0; s < steps && !rc; s++) {
+        NsArgs g = a;      /* A = X X^T */
+        g.A = g.B = X; g.out = g.out_t = A;
+        g.KB = wp / 16; g.KU = (u32)(round_up(w, 64) / 16); g.KBO = g.KBT = np / 16;
+        g.tm = g.tn = tn; g.sym = 1; g.beta = 1.0f / 16384;
+        rc = launch1(name, half, 1, count, lanes, &g);
+        g.A = g.B = g.old = A; g.out = g.out_t = B;      /* B = b A + c A A */
+        g.KB = np / 16; g.KU = (u32)(round_up(n, 64) / 16);
+        g.alpha = (f32)(NS_B / 2); g.beta = (f32)(NS_C / 32768);
+        if (!rc) rc = launch1(name, half, 1, count, lanes, &g);
+        g.A = B; g.B = xt; g.old = X;                    /* X = a X + B X */
+        g.KBO = wp / 16; g.sym = 0; g.tn = tw;
+        g.last = s + 1 == steps;
+        g.out = g.last ? 0 : X; g.out_t = g.last ? 0 : xt2;
+        g.alpha = (f32)(g.last ? NS_A / 16384 : NS_A); g.beta = g.last ? 1.0f / (1 << 27) : 1.0f / 8192;
+        if (!rc) rc = launch1(name, (u64)tn * tw, 1, count, lanes, &g);
+        const u64 t = xt; xt = xt2; xt2 = t;
+    }
+    return rc;
+}
+
+int thvm_hip_muon_step(const u32 *param, const u32 *grad, const u32 *m, u32 count, u32 rows, u32 cols, f32 lr, f32 scale,
+                       f32 weight_decay, f32 beta, u32 nesterov, u32 steps, u32 dtype) {
+    if (!hipb.initialized) return THVM_HIP_EINVAL;
+    const char *op = "muon_step";
+    if (!dtype_ok(dtype)) return refuse(op, "the type is neither f32 nor f16");
+    if (!steps || steps > 64) return refuse(op, "1 to 64 Newton-Schulz steps are possible");
+    if (count && (!param || !grad || !m)) return refuse(op, "no parameters, gradients or momenta");
+    const u64 numel = (u64)rows * cols, es = esize(dtype);
+    for (u32 i = 0; i < count; i++) {
+        if (!param[i] || !grad[i] || !m[i]) return refuse(op, "no parameter, gradient or momentum");
+        const Operand o[] = {{param[i], numel * es, 1}, {m[i], numel * 4, 1}, {grad[i], numel * es, 0}};
+        if (!operands_ok(op, o, 3, NULL, 0)) return THVM_HIP_EINVAL;
+        for (u32 j = 0; j < i; j++)
+            if (param[j] == param[i] || m[j] == m[i] || param[j] == m[i] || m[j] == param[i] || param[j] == grad[i] ||
+                grad[j] == param[i] || m[j] == grad[i] || grad[j] == m[i])
+                return refuse(op, "an output is also another operand");
+    }
+    if (!numel || !count) return THVM_HIP_OK;
+    const u32 cu = hipb.n_cu ? hipb.n_cu : 256;
+    u32 tile = 256;
+    while (tile > 64 && count * div_up(rows, tile) * div_up(cols, tile) < cu * 3 / 4) tile /= 2;
+    const u64 n = round_up(rows < cols ? rows : cols, tile), w = round_up(rows < cols ? cols : rows, tile);
+    const u64 each = (dtype == DTYPE_F16 ? 2ull : 4ull) * (3 * n * w + 2 * n * n);
+    /* as many matrices at once as a launch names, in 4 GiB of workspace */
+    u64 at_once = (4ull << 30) / each;
+    if (at_once < 1) at_once = 1;
+    if (at_once > MUON_MAX) at_once = MUON_MAX;
+    const f32 keep = (f32)(1.0 - (double)lr * weight_decay), step = (f32)((double)lr * scale);
+    int rc = THVM_HIP_OK;
+    for (u32 i = 0; i < count && !rc; i += (u32)at_once) {
+        const u32 nc = count - i < at_once ? count - i : (u32)at_once;
+        for (u32 j = i; j < i + nc; j++) hipb_operand(param[j]), hipb_operand(grad[j]), hipb_operand(m[j]);
+        rc = muon_chunk(param + i, grad + i, m + i, nc, rows, cols, keep, step, beta, nesterov != 0, steps, dtype, tile);
+        for (u32 j = i; j < i + nc; j++) pool_mark_device_write(param[j]), pool_mark_device_write(m[j]);
+    }
+    return rc;
+}
