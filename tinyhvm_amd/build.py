@@ -57,6 +57,7 @@ def _embed(source):
         for i in range(0, len(data), 24):
             f.write("  " + ",".join(str(b) for b in data[i:i + 24]) + ",\n")
         f.write("};\n")
+        f.write("const unsigned long thvm_%s_co_len = %dUL;\n" % (name, len(data)))
     return blob
 
 

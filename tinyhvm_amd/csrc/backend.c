@@ -1346,6 +1346,7 @@ static int hb_init(void) {
         *(volatile u32 *)hipb.comb_err_host = 0;
     }
     if (rtc_init() != 0) return -1;
+    if (block_init && block_init() != 0) return -1;
     /* the single-pass combine area, zeroed once by a kernel */
     {
         u64 c1 = 0;
@@ -1378,7 +1379,7 @@ static void hb_shutdown(void) {
     graphs_release_all();
     dense_shutdown();
     window_shutdown();
-    block_shutdown();
+    if (block_shutdown) block_shutdown();
     hb_release();
     upload_release();
     rtc_shutdown();

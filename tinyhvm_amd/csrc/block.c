@@ -8,14 +8,66 @@
  */
 #include <math.h>
 #include <string.h>
+#include <stdlib.h>
 
 #include "hipb.h"
 #include "thvm_hip.h"
 #include "block_args.h"
 
+extern const unsigned char thvm_norm_kernels_co[], thvm_gemm_kernels_co[];
+
+#define MODULES 2
+#define KERNELS 256 /* more than the modules have */
+static struct {
+    hipModule_t mod[MODULES];
+    struct { char name[48]; hipFunction_t fn; } fn[KERNELS];
+} B;
 static Scratch block_ws;
 
-void block_shutdown(void) { scratch_release(&block_ws); }
+void block_shutdown(void) {
+    scratch_release(&block_ws);
+    for (int i = 0; i < MODULES; i++)
+        if (B.mod[i]) HIPB_CHECK(hipModuleUnload(B.mod[i]));
+    memset(&B, 0, sizeof B);
+}
+
+int block_init(void) {
+    const unsigned char *co[MODULES] = {thvm_norm_kernels_co, thvm_gemm_kernels_co};
+    memset(&B, 0, sizeof B);
+    for (int i = 0; i < MODULES; i++) {
+        hipError_t e = hipModuleLoadData(&B.mod[i], co[i]);
+        if (e != hipSuccess) {
+            fprintf(stderr, "tinyhvm-hip: loading an operator module failed: %s\n", hipGetErrorString(e));
+            B.mod[i] = NULL;
+            return -1;
+        }
+    }
+    return 0;
+}
+
+/* A kernel by name, looked up in the modules once. */
+static hipFunction_t kernel(const char *name) {
+    u32 h = 2166136261u;
+    for (const char *c = name; *c; c++) h = (h ^ (u8)*c) * 16777619u;
+    for (u32 p = h % KERNELS, n = 0; n < KERNELS; p = (p + 1) % KERNELS, n++) {
+        if (B.fn[p].name[0] && strcmp(B.fn[p].name, name) != 0) continue;
+        if (B.fn[p].name[0]) return B.fn[p].fn;
+        hipFunction_t f = NULL;
+        for (int i = 0; i < MODULES && !f; i++)
+            if (hipModuleGetFunction(&f, B.mod[i], name) != hipSuccess) {
+                (void)hipGetLastError(); /* it may be in the next module: no error of this thread's */
+                f = NULL;
+            }
+        if (!f) {
+            fprintf(stderr, "tinyhvm-hip: kernel %s not found\n", name);
+            return NULL;
+        }
+        snprintf(B.fn[p].name, sizeof B.fn[p].name, "%s", name);
+        B.fn[p].fn = f;
+        return f;
+    }
+    return NULL;
+}
 
 /* ---- arguments ---- */
 
@@ -71,7 +123,7 @@ static int launch(const char *name, u64 gx, u32 gy, u32 gz, u32 bx, void **param
         fprintf(stderr, "tinyhvm-hip: %s: the grid exceeds the launch limit\n", name);
         return THVM_HIP_EINVAL;
     }
-    hipFunction_t fn = rtc_static_fn(name);
+    hipFunction_t fn = kernel(name);
     if (!fn || !hipb_launch(fn, (u32)gx, gy, gz, bx, params)) return THVM_HIP_EDEVICE;
     return THVM_HIP_OK;
 }
@@ -209,7 +261,7 @@ static Packed packed_of(u32 rows, u32 k, u32 tile) {
 }
 
 static void packed_carve(Packed *p, Carve *c, u32 dtype) {
-    p->p = carve(c, packed_bytes(p, dtype));
+    p->p = carve(c, packed_bytes(p, dtype) + PACK_SLACK);
     p->e = carve(c, dtype == DTYPE_F32 ? p->Rp * 4ull : 0);
 }
 
@@ -226,8 +278,10 @@ static Plan plan_of(u32 M, u32 N, u32 K, u32 dtype) {
         p.tn = (u32)div_up(N, p.tile);
         if ((u64)p.tm * p.tn >= cu * 3 / 4) break;
     }
-    const u64 tiles = (u64)p.tm * p.tn, stages = round_up(K, 64) / (dtype == DTYPE_F16 ? 64 : 32);
-    while (tiles * p.splits * 2 <= cu * 2 && stages / (p.splits * 2) >= 4 && p.splits < 16) p.splits *= 2;
+    /* workgroups that the card holds at once: LDS is one 256 tile's, or two of the others' */
+    const u64 tiles = (u64)p.tm * p.tn, slots = p.tile == 256 ? cu : 2 * cu, chunks = round_up(K, 64) / 64;
+    while (tiles * p.splits * 2 <= slots && chunks / (p.splits * 2) >= 4 && p.splits < 16) p.splits *= 2;
+    if (getenv("PLANX")) { int t, sp; sscanf(getenv("PLANX"), "%d,%d", &t, &sp); p.tile = t; p.tm = div_up(M, t); p.tn = div_up(N, t); p.splits = sp; }
     return p;
 }
 
@@ -445,7 +499,7 @@ static int muon_chunk(const u32 *param, const u32 *grad, const u32 *m, u32 count
     u64 ops = 0;
     Carve c = {0, 0};
     for (int pass = 0; pass < 2; pass++) {
-        ops = carve(&c, stride * count);
+        ops = carve(&c, stride * count + PACK_SLACK);
         mu.sums = carve(&c, 8ull * mu.blocks * count);
         if (!pass && !carve_reserve(&c)) return THVM_HIP_ENOMEM;
     }

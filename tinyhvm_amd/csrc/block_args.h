@@ -25,6 +25,9 @@ typedef struct {
 /* activations: THVM_HIP_ACT_* */
 enum { ACT_NONE = 0, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU, ACT_COUNT };
 
+/* bytes past a packed operand that a product's last loads may touch */
+#define PACK_SLACK 16384
+
 /* C[M][N] = sum over k of A[r][k] B[c][k], packed operands (gemm_kernels.hip) */
 typedef struct {
     u64 A, B;                  /* packed; KB blocks of 16 k */

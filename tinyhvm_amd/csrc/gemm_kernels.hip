@@ -24,25 +24,35 @@
 #include <hip/hip_runtime.h>
 #include "thvm_abi.h"
 #include "block_args.h"
+#include "block_mem.h"
 
-typedef _Float16 f16;
 typedef f16 h8 __attribute__((ext_vector_type(8)));
 typedef float f16v __attribute__((ext_vector_type(16)));   // a 32x32 block's sums
 typedef float f4 __attribute__((ext_vector_type(4)));
-template <typename T, u32 N> struct __attribute__((packed, aligned(sizeof(T)))) Pack { T v[N]; };
 
 // ---- activations (thvm_hip.h) ----
 
-__device__ __forceinline__ float sigmoid(float z) { return 1.0f / (1.0f + __expf(-z)); }
+__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + __expf(-z)); }
 
 // gelu's tanh form is z * sigmoid(2 sqrt(2/pi) (z + 0.044715 z^3))
 #define GELU_U 1.5957691216057308f
 #define GELU_C 0.044715f
 
+// The normal distribution's integral up to z, by the rational approximation of
+// erfc in Abramowitz and Stegun, 7.1.26: within 7.5e-8, a third of the
+// instructions of erff. Taken on the side of the small tail, so that a tail is
+// a small number and not what is left of 1.
+__device__ __forceinline__ float normal_cdf(float z) {
+    const float x = fabsf(z) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * x);
+    const float p = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+    const float tail = 0.5f * p * __expf(-x * x);
+    return z < 0.0f ? tail : 1.0f - tail;
+}
+
 __device__ __forceinline__ float act_of(u32 act, float z) {
     switch (act) {
     case ACT_RELU: return z > 0.0f ? z : 0.0f;
-    case ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+    case ACT_GELU: return z * normal_cdf(z);
     case ACT_GELU_TANH: return z * sigmoid(GELU_U * (z + GELU_C * z * z * z));
     case ACT_SILU: return z * sigmoid(z);
     default: return z;
@@ -55,8 +65,7 @@ __device__ __forceinline__ float act_slope(u32 act, float z) {
     const float near = fminf(fmaxf(z, -128.0f), 128.0f);
     switch (act) {
     case ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
-    case ACT_GELU:
-        return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + near * (0.3989422804014327f * __expf(-0.5f * near * near));
+    case ACT_GELU: return normal_cdf(z) + near * (0.3989422804014327f * __expf(-0.5f * near * near));
     case ACT_GELU_TANH: {
         const float s = sigmoid(GELU_U * (z + GELU_C * z * z * z));
         return s + near * (s * (1.0f - s)) * (GELU_U * (1.0f + 3.0f * GELU_C * near * near));
@@ -69,33 +78,24 @@ __device__ __forceinline__ float act_slope(u32 act, float z) {
     }
 }
 
-// ---- 8 consecutive elements of a row, zeros past its end ----
-
-template <typename T>
-__device__ __forceinline__ void load8(const T *row, u32 e, u32 n, float *out) {
-    if (e + 8 <= n) {
-        const Pack<T, 8> p = *(const Pack<T, 8> *)(row + e);
-#pragma unroll
-        for (u32 j = 0; j < 8; j++) out[j] = (float)p.v[j];
-    } else {
-#pragma unroll
-        for (u32 j = 0; j < 8; j++) out[j] = e + j < n ? (float)row[e + j] : 0.0f;
+// The same of 8 values: one choice for all of them.
+#define ACT_CASES(f, ...)                                                                                          \
+    switch (act) {                                                                                                 \
+    case ACT_RELU: ACT_EACH(f(ACT_RELU, z[j]), __VA_ARGS__) break;                                                 \
+    case ACT_GELU: ACT_EACH(f(ACT_GELU, z[j]), __VA_ARGS__) break;                                                 \
+    case ACT_GELU_TANH: ACT_EACH(f(ACT_GELU_TANH, z[j]), __VA_ARGS__) break;                                       \
+    case ACT_SILU: ACT_EACH(f(ACT_SILU, z[j]), __VA_ARGS__) break;                                                 \
+    default: break;                                                                                                \
     }
+#define ACT_EACH(e, op) _Pragma("unroll") for (u32 j = 0; j < 8; j++) v[j] op e;
+__device__ __forceinline__ void act8(u32 act, float *v) {
+    const float *z = v;
+    ACT_CASES(act_of, =)
 }
+__device__ __forceinline__ void slope8(u32 act, const float *z, float *v) { ACT_CASES(act_slope, *=) }
 
-template <typename T>
-__device__ __forceinline__ void store8(T *row, u32 e, u32 n, const float *in) {
-    if (e + 8 <= n) {
-        Pack<T, 8> p;
-#pragma unroll
-        for (u32 j = 0; j < 8; j++) p.v[j] = (T)in[j];
-        *(Pack<T, 8> *)(row + e) = p;
-    } else {
-#pragma unroll
-        for (u32 j = 0; j < 8; j++)
-            if (e + j < n) row[e + j] = (T)in[j];
-    }
-}
+template <typename T> __device__ __forceinline__ void load8(const glob<T> *row, u32 e, u32 n, float *out) { load_n<T, 8>(row, e, n, out); }
+template <typename T> __device__ __forceinline__ void store8(glob<T> *row, u32 e, u32 n, const float *in) { store_n<T, 8>(row, e, n, in); }
 
 // ---- packed operands ----
 
@@ -116,7 +116,7 @@ __device__ __forceinline__ bool exp_marked(int w) { return ((w >> 30) & 1) != ((
 
 // The sum of a row's products with the planes as they are, in 32 bits.
 template <u32 PL>
-__device__ __noinline__ float exact_dot(const f16 *A, const f16 *B, u32 KB, u32 r, u32 c) {
+__device__ __forceinline__ float exact_dot(const glob<f16> *A, const glob<f16> *B, u32 KB, u32 r, u32 c) {
     float s = 0.0f;
     for (u32 kb = 0; kb < KB; kb++)
         for (u32 t = 0; t < 16; t++) {
@@ -135,31 +135,43 @@ __device__ __noinline__ float exact_dot(const f16 *A, const f16 *B, u32 KB, u32 
 typedef __attribute__((address_space(1))) const void *gptr;
 typedef __attribute__((address_space(3))) void *lptr;
 
-// every DMA but the last n of this wave has landed, and every wave is here
-template <u32 n> __device__ __forceinline__ void wait_stage() {
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(n) : "memory");
+// Every load to LDS but the last `loads` of this wave and every read of LDS
+// but the last `reads` are done, and every wave is here.
+template <u32 loads, u32 reads> __device__ __forceinline__ void wait_stage() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(%1)\n\ts_barrier" ::"n"(loads), "n"(reads) : "memory");
 }
 
-// A tile of TM x TN by WM x WN waves. A stage is 64 / PL of K: 4 KB of each
-// row block, the same chunks that lie together in memory. NS stages of LDS:
-// NS - 1 are on their way or in use while the last one is multiplied.
-template <u32 TM_, u32 TN_, u32 WM_, u32 WN_, u32 PL_, u32 NS_>
+// A tile of TM x TN by WM x WN waves. A unit is one k step of the matrix
+// instruction over all planes; a stage is US units, the chunks of each row
+// block that lie together in memory. LDS holds NS stages. Small tiles have
+// longer stages: a barrier then stands between enough multiplications.
+template <u32 TM_, u32 TN_, u32 WM_, u32 WN_, u32 PL_, u32 US_, u32 NS_>
 struct Tile {
-    static constexpr u32 TM = TM_, TN = TN_, WM = WM_, WN = WN_, PL = PL_, NS = NS_;
+    static constexpr u32 TM = TM_, TN = TN_, WM = WM_, WN = WN_, PL = PL_, US = US_, NS = NS_;
     static constexpr u32 WAVES = WM * WN, THREADS = WAVES * 64, RBA = TM / 32, RBB = TN / 32, RB = RBA + RBB;
-    static constexpr u32 MI = TM / WM / 32, NI = TN / WN / 32, KS = 4 / PL;
-    static constexpr u32 STAGE = RB * 2048;                 // f16 elements
+    static constexpr u32 MI = TM / WM / 32, NI = TN / WN / 32;
+    static constexpr u32 CK = US * PL;                      // chunks of a row block in a stage
+    static constexpr u32 STAGE = RB * CK * 512;             // f16 elements
     static constexpr u32 PITCH = NI * 32 + 4;               // the epilogue's staging rows
     static constexpr u32 EPI = WAVES * 32 * PITCH * 2;      // f16 elements
     static constexpr u32 LDS = NS * STAGE > EPI ? NS * STAGE : EPI;
-    static constexpr u32 CH = RB * 4 / WAVES;               // chunks a wave brings in a stage
-    static_assert(RB * 4 % WAVES == 0 && CH % 4 == 0, "a wave brings whole row blocks");
+    static constexpr u32 Q = RB / WAVES, CH = Q * CK;       // row blocks and chunks a wave brings in a stage
+    static constexpr u32 READS = (MI + NI) * CK;            // fragments a wave reads of a stage
+    static constexpr u32 TURN = US == 1 ? 2 : 1;            // stages a turn of the main loop
+    static_assert(READS < 16 && RB % WAVES == 0 && (NS & (NS - 1)) == 0 && CK <= 4 && (US == 1 || US % 2 == 0),
+                  "a wave brings whole row blocks; units alternate between two sets of registers");
+    static_assert((NS - 1) * CK * 1024 <= PACK_SLACK, "loads past the end");
 };
 
+// The sums of a tile over stages s0 .. s1 - 1. A unit's fragments are read
+// from LDS while the unit before is multiplied; where that begins a stage,
+// the wait for the stage and the barrier come ahead of the reads, so that
+// they too pass behind multiplications. A stage is brought NS - 1 ahead, into
+// the buffer whose last reader has passed that barrier.
 template <typename TL>
-__device__ __forceinline__ void mainloop(f16 *lds, const f16 *A, const f16 *B, u32 KBA, u32 KBB, u32 rb0, u32 cb0, u32 s0, u32 s1,
+__device__ __forceinline__ void mainloop(f16 *lds, const glob<f16> *A, const glob<f16> *B, u32 KBA, u32 KBB, u32 rb0, u32 cb0, u32 s0, u32 s1,
                                          f16v (&acc)[TL::MI][TL::NI]) {
-    constexpr u32 PL = TL::PL, NS = TL::NS, Q = TL::CH / 4;    // Q: row blocks this wave brings
+    constexpr u32 PL = TL::PL, NS = TL::NS, Q = TL::Q;
     const u32 lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const u32 wm = wave / TL::WN, wn = wave % TL::WN;
 #pragma unroll
@@ -169,57 +181,75 @@ __device__ __forceinline__ void mainloop(f16 *lds, const f16 *A, const f16 *B, u
 #pragma unroll
             for (u32 v = 0; v < 16; v++) acc[i][j][v] = 0.0f;
     if (s0 >= s1) return;
-    const f16 *src[Q];
+    const glob<f16> *src[Q];
 #pragma unroll
     for (u32 q = 0; q < Q; q++) {
         const u32 b = wave * Q + q;
-        const f16 *base = b < TL::RBA ? A + block_at<PL>(rb0 + b, 0, KBA, 0) : B + block_at<PL>(cb0 + b - TL::RBA, 0, KBB, 0);
-        src[q] = base + (u64)s0 * 2048u + lane * 8u;
+        const glob<f16> *base = b < TL::RBA ? A + block_at<PL>(rb0 + b, 0, KBA, 0) : B + block_at<PL>(cb0 + b - TL::RBA, 0, KBB, 0);
+        src[q] = base + (u64)s0 * (TL::CK * 512u) + lane * 8u;
     }
-    // Past the last stage it is brought again, into a buffer that nothing
-    // reads any more, so that the count of loads in flight stays the same.
-    u32 next = s0;
+    // Past the last stage what follows in memory is brought, for no one to
+    // read, so that the count of loads in flight stays the same (a packed
+    // operand ends PACK_SLACK short of its allocation).
     auto bring = [&](u32 buf) {
 #pragma unroll
         for (u32 q = 0; q < Q; q++) {
-            const u32 dst = (u32)(uintptr_t)(lptr)lds + (buf * TL::STAGE + (wave * Q + q) * 2048u) * 2u;
-#define BRING(c) __builtin_amdgcn_global_load_lds((gptr)src[q], (lptr)(uintptr_t)dst, 16, c * 1024, 0);
+            const u32 dst = (u32)(uintptr_t)(lptr)lds + (buf * TL::STAGE + (wave * Q + q) * (TL::CK * 512u)) * 2u;
+#define BRING(c) if (c < TL::CK) __builtin_amdgcn_global_load_lds((gptr)src[q], (lptr)(uintptr_t)dst, 16, c * 1024, 0);
             BRING(0) BRING(1) BRING(2) BRING(3)
 #undef BRING
-            if (next + 1 < s1) src[q] += 2048;
+            src[q] += TL::CK * 512u;
         }
-        next++;
     };
-#pragma unroll
-    for (u32 i = 0; i + 1 < NS; i++) bring(i);
-    for (u32 s = s0, buf = 0, nb = NS - 1; s < s1; s++) {
-        wait_stage<(NS - 2) * TL::CH>();
-        bring(nb);
+    h8 a[2][TL::MI][PL], b[2][TL::NI][PL];
+    auto fetch = [&](u32 buf, u32 k, h8 (&fa)[TL::MI][PL], h8 (&fb)[TL::NI][PL]) {
         const f16 *st = lds + buf * TL::STAGE + lane * 8u;
 #pragma unroll
-        for (u32 k = 0; k < TL::KS; k++) {
-            h8 a[TL::MI][PL], b[TL::NI][PL];
+        for (u32 p = 0; p < PL; p++) {
 #pragma unroll
-            for (u32 p = 0; p < PL; p++) {
+            for (u32 j = 0; j < TL::NI; j++) fb[j][p] = *(const h8 *)(st + ((TL::RBA + wn * TL::NI + j) * TL::CK + k * PL + p) * 512u);
 #pragma unroll
-                for (u32 i = 0; i < TL::MI; i++) a[i][p] = *(const h8 *)(st + ((wm * TL::MI + i) * 4 + k * PL + p) * 512u);
+            for (u32 i = 0; i < TL::MI; i++) fa[i][p] = *(const h8 *)(st + ((wm * TL::MI + i) * TL::CK + k * PL + p) * 512u);
+        }
+    };
+    auto multiply = [&](const h8 (&fa)[TL::MI][PL], const h8 (&fb)[TL::NI][PL]) {
 #pragma unroll
-                for (u32 j = 0; j < TL::NI; j++)
-                    b[j][p] = *(const h8 *)(st + ((TL::RBA + wn * TL::NI + j) * 4 + k * PL + p) * 512u);
-            }
+        for (u32 t = 0; t < 2 * PL - 1; t++)       // hi hi, then hi lo and lo hi
 #pragma unroll
             for (u32 i = 0; i < TL::MI; i++)
 #pragma unroll
-                for (u32 j = 0; j < TL::NI; j++) {
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][0], b[j][0], acc[i][j], 0, 0, 0);
-                    if (PL == 2) {
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][0], b[j][PL - 1], acc[i][j], 0, 0, 0);
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][PL - 1], b[j][0], acc[i][j], 0, 0, 0);
-                    }
-                }
+                for (u32 j = 0; j < TL::NI; j++)
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[i][t >> 1], fb[j][t & 1], acc[i][j], 0, 0, 0);
+    };
+    // One of the next unit's fragments is read after each of the first
+    // multiplications: left alone, the compiler puts the reads last.
+    auto unit = [&](u32 buf, u32 k, const h8 (&fa)[TL::MI][PL], const h8 (&fb)[TL::NI][PL], h8 (&na)[TL::MI][PL],
+                    h8 (&nb)[TL::NI][PL]) {
+        __builtin_amdgcn_sched_barrier(0);
+        fetch(buf, k, na, nb);
+        multiply(fa, fb);
+#pragma unroll
+        for (u32 i = 0; i < (TL::MI + TL::NI) * PL; i++) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
-        nb = buf;
-        buf = buf + 1 == NS ? 0 : buf + 1;
+        __builtin_amdgcn_sched_barrier(0);
+    };
+#pragma unroll
+    for (u32 i = 0; i + 1 < NS; i++) bring(i);
+    wait_stage<(NS - 2) * TL::CH, 0>();
+    fetch(0, 0, a[0], b[0]);
+    for (u32 s = s0, buf = 0; s < s1; s += TL::TURN) {
+#pragma unroll
+        for (u32 u = 0; u < TL::US * TL::TURN; u++) {
+            const bool fresh = (u + 1) % TL::US == 0;       // the next unit begins a stage
+            if (fresh) {
+                wait_stage<(NS - 3) * TL::CH, TL::READS>();
+                bring((buf + NS - 1) & (NS - 1));
+                buf = (buf + 1) & (NS - 1);
+            }
+            unit(buf, fresh ? 0 : u + 1, a[u & 1], b[u & 1], a[(u + 1) & 1], b[(u + 1) & 1]);
+        }
     }
 }
 
@@ -242,12 +272,10 @@ __device__ __forceinline__ void tile_upper(u32 t, u32 &i, u32 &j) {
     i = t - j * (j + 1) / 2;
 }
 
-// One wave's sums of a 32-row block, through LDS: f(r, c, v) is called with 8
-// consecutive columns c.. of row r (in the tile), a wave's lanes side by side.
-template <typename TL, typename F>
-__device__ __forceinline__ void by_rows(float *st, const f16v (&acc)[TL::NI], F f) {
+// One wave's sums of a 32-row block into LDS, for its lanes to take rows of.
+template <typename TL>
+__device__ __forceinline__ void stage_rows(float *st, const f16v (&acc)[TL::NI]) {
     const u32 lane = threadIdx.x & 63u;
-    constexpr u32 LPR = TL::NI * 4, RPP = 64 / LPR;
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (u32 j = 0; j < TL::NI; j++)
@@ -255,14 +283,6 @@ __device__ __forceinline__ void by_rows(float *st, const f16v (&acc)[TL::NI], F 
         for (u32 v = 0; v < 16; v++) st[((v >> 2) * 8 + (lane >> 5) * 4 + (v & 3)) * TL::PITCH + j * 32 + (lane & 31u)] = acc[j][v];
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-#pragma unroll
-    for (u32 p = 0; p < 32 / RPP; p++) {
-        const u32 r = p * RPP + lane / LPR, c = (lane % LPR) * 8;
-        float v[8];
-        *(f4 *)v = *(const f4 *)(st + r * TL::PITCH + c);
-        *(f4 *)(v + 4) = *(const f4 *)(st + r * TL::PITCH + c + 4);
-        f(r, c, v);
-    }
 }
 
 // What an output becomes: z = sum (+ bias), y = act(z) (+ residual).
@@ -270,34 +290,43 @@ template <typename T>
 __device__ __forceinline__ void finish8(const GemmArgs &a, u32 r, u32 c, float *v) {
     float t[8];
     if (a.bias) {
-        load8<T>((const T *)a.bias, c, a.N, t);
+        load8<T>((const glob<T> *)a.bias, c, a.N, t);
 #pragma unroll
         for (u32 j = 0; j < 8; j++) v[j] += t[j];
     }
-    if (a.z) store8<T>((T *)a.z + (u64)r * a.N, c, a.N, v);
-    if (a.act)
-#pragma unroll
-        for (u32 j = 0; j < 8; j++) v[j] = act_of(a.act, v[j]);
+    if (a.z) store8<T>((glob<T> *)a.z + (u64)r * a.N, c, a.N, v);
+    act8(a.act, v);
     if (a.res) {
-        load8<T>((const T *)a.res + (u64)r * a.N, c, a.N, t);
+        load8<T>((const glob<T> *)a.res + (u64)r * a.N, c, a.N, t);
 #pragma unroll
         for (u32 j = 0; j < 8; j++) v[j] += t[j];
     }
-    store8<T>((T *)a.out + (u64)r * a.N, c, a.N, v);
+    store8<T>((glob<T> *)a.out + (u64)r * a.N, c, a.N, v);
 }
 
-// The sums of 32-bit operands at their own scale.
-template <u32 PL>
-__device__ __forceinline__ void unscale8(const GemmArgs &a, u32 r, u32 c, float *v) {
-    if (PL == 1) return;
-    const int er = ((const int *)a.ea)[r];
+// One output whose row or column is marked, its sum computed again.
+template <u32 PL, typename T>
+__device__ __forceinline__ void finish_marked(const GemmArgs &a, u32 r, u32 c) {
+    const int e = exp_of(((const glob<int> *)a.ea)[r]) + exp_of(((const glob<int> *)a.eb)[c]);
+    float v = ldexpf(exact_dot<PL>((const glob<f16> *)a.A, (const glob<f16> *)a.B, a.KB, r, c), -e);
+    const u64 at = (u64)r * a.N + c;
+    if (a.bias) v += (float)((const glob<T> *)a.bias)[c];
+    if (a.z) ((glob<T> *)a.z)[at] = (T)v;
+    v = act_of(a.act, v);
+    if (a.res) v += (float)((const glob<T> *)a.res)[at];
+    ((glob<T> *)a.out)[at] = (T)v;
+}
+
+// The exponents of 8 columns (padded to whole tiles), and whether one is marked.
+__device__ __forceinline__ bool column_exps(const GemmArgs &a, u32 c, int *ec) {
+    bool odd = false;
 #pragma unroll
     for (u32 j = 0; j < 8; j++) {
-        const int ec = ((const int *)a.eb)[c + j];    // padded to whole tiles
-        if ((exp_marked(er) || exp_marked(ec)) && c + j < a.N)
-            v[j] = exact_dot<PL>((const f16 *)a.A, (const f16 *)a.B, a.KB, r, c + j);
-        v[j] = ldexpf(v[j], -(exp_of(er) + exp_of(ec)));
+        const int w = ((const glob<int> *)a.eb)[c + j];
+        odd |= exp_marked(w);
+        ec[j] = exp_of(w);
     }
+    return odd;
 }
 
 // A tile of one product, or of one of its K splits (blockIdx.y): the partial
@@ -307,26 +336,92 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs &a, f16 *lds) {
     const u32 wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     u32 ti, tj;
     tile_of(blockIdx.x, a.tm, a.tn, ti, tj);
-    const u32 S = a.KB / TL::KS, per = (S + a.splits - 1) / a.splits, s0 = blockIdx.y * per;
+    const u32 S = a.KB / TL::US, per = (S / TL::TURN + a.splits - 1) / a.splits * TL::TURN, s0 = blockIdx.y * per;
     const u32 s1 = s0 + per < S ? s0 + per : S;
     f16v acc[TL::MI][TL::NI];
-    mainloop<TL>(lds, (const f16 *)a.A, (const f16 *)a.B, a.KB, a.KB, ti * TL::RBA, tj * TL::RBB, s0, s1, acc);
-    wait_stage<0>();
+    mainloop<TL>(lds, (const glob<f16> *)a.A, (const glob<f16> *)a.B, a.KB, a.KB, ti * TL::RBA, tj * TL::RBB, s0, s1, acc);
+    wait_stage<0, 0>();
+    // A lane keeps 8 columns and takes every RPP-th row of them. The residual
+    // of a 32-row block is asked for before the block ahead of it is finished.
+    constexpr u32 LPR = TL::NI * 4, RPP = 64 / LPR, PASSES = 32 / RPP;
+    const u32 lane = threadIdx.x & 63u, dc = (lane % LPR) * 8, c = tj * TL::TN + (wave % TL::WN) * TL::NI * 32 + dc;
+    const u32 r0 = ti * TL::TM + (wave / TL::WN) * TL::MI * 32 + lane / LPR;
     float *st = (float *)lds + wave * 32 * TL::PITCH;
+    const float *row = st + (lane / LPR) * TL::PITCH + dc;
+    if (a.splits > 1) {
+#pragma unroll
+        for (u32 i = 0; i < TL::MI; i++) {
+            stage_rows<TL>(st, acc[i]);
+#pragma unroll
+            for (u32 p = 0; p < PASSES; p++) {
+                const u32 r = r0 + i * 32 + p * RPP;
+                float v[8];
+                *(f4 *)v = *(const f4 *)(row + p * RPP * TL::PITCH);
+                *(f4 *)(v + 4) = *(const f4 *)(row + p * RPP * TL::PITCH + 4);
+                if (r < a.M && c < a.N) store8<float>((glob<float> *)a.part + ((u64)blockIdx.y * a.M + r) * a.N, c, a.N, v);
+            }
+        }
+        return;
+    }
+    const bool whole = c + 8 <= a.N;
+    float bias[8];
+    int ec[8];
+    bool odd = false, left = false;      // a column that is marked; outputs left for later
+    if (a.bias) load8<T>((const glob<T> *)a.bias, c, a.N, bias);
+    if (TL::PL == 2) odd = column_exps(a, c, ec);
+    any_vec<T, 8> res[2][PASSES];
+    auto ask = [&](u32 i, any_vec<T, 8> (&x)[PASSES]) {
+#pragma unroll
+        for (u32 p = 0; p < PASSES; p++) {
+            const u32 r = r0 + i * 32 + p * RPP;
+            if (a.res && whole && r < a.M) x[p] = *(const glob<any_vec<T, 8>> *)((const glob<T> *)a.res + (u64)r * a.N + c);
+        }
+    };
+    ask(0, res[0]);
 #pragma unroll
     for (u32 i = 0; i < TL::MI; i++) {
-        const u32 r0 = ti * TL::TM + ((wave / TL::WN) * TL::MI + i) * 32, c0 = tj * TL::TN + (wave % TL::WN) * TL::NI * 32;
-        by_rows<TL>(st, acc[i], [&](u32 dr, u32 dc, float *v) {
-            const u32 r = r0 + dr, c = c0 + dc;
-            if (r >= a.M || c >= a.N) return;
-            if (a.splits > 1) {
-                store8<float>((float *)a.part + ((u64)blockIdx.y * a.M + r) * a.N, c, a.N, v);
-                return;
+        if (i + 1 < TL::MI) ask(i + 1, res[(i + 1) & 1]);
+        stage_rows<TL>(st, acc[i]);
+#pragma unroll
+        for (u32 p = 0; p < PASSES; p++) {
+            const u32 r = r0 + i * 32 + p * RPP;
+            if (r >= a.M || c >= a.N) continue;
+            float v[8];
+            *(f4 *)v = *(const f4 *)(row + p * RPP * TL::PITCH);
+            *(f4 *)(v + 4) = *(const f4 *)(row + p * RPP * TL::PITCH + 4);
+            if (TL::PL == 2) {
+                const int er = ((const glob<int> *)a.ea)[r];
+                if (odd || exp_marked(er)) {
+                    left = true;
+                    continue;
+                }
+#pragma unroll
+                for (u32 j = 0; j < 8; j++) v[j] = ldexpf(v[j], -(er + ec[j]));
             }
-            unscale8<TL::PL>(a, r, c, v);
-            finish8<T>(a, r, c, v);
-        });
+            if (a.bias)
+#pragma unroll
+                for (u32 j = 0; j < 8; j++) v[j] += bias[j];
+            const u64 at = (u64)r * a.N;
+            if (a.z) store8<T>((glob<T> *)a.z + at, c, a.N, v);
+            act8(a.act, v);
+            if (a.res) {
+                if (whole)
+#pragma unroll
+                    for (u32 j = 0; j < 8; j++) v[j] += (float)res[i & 1][p][j];
+                else
+#pragma unroll
+                    for (u32 j = 0; j < 8; j++)
+                        if (c + j < a.N) v[j] += (float)((const glob<T> *)a.res)[at + c + j];
+            }
+            store8<T>((glob<T> *)a.out + at, c, a.N, v);
+        }
     }
+    if (TL::PL == 2 && left)
+        for (u32 q = 0; q < TL::MI * PASSES; q++) {
+            const u32 r = r0 + q * RPP;
+            if (r < a.M && (odd || exp_marked(((const glob<int> *)a.ea)[r])))
+                for (u32 j = 0; j < 8 && c + j < a.N; j++) finish_marked<TL::PL, T>(a, r, c + j);
+        }
 }
 
 // The sums of K splits, in split order, and what an output becomes.
@@ -338,11 +433,20 @@ __device__ __forceinline__ void gemm_join(const GemmArgs &a) {
     const u32 r = (u32)(t / per), c = (u32)(t % per) * 8;
     float v[8] = {0, 0, 0, 0, 0, 0, 0, 0}, p[8];
     for (u32 s = 0; s < a.splits; s++) {
-        load8<float>((const float *)a.part + ((u64)s * a.M + r) * a.N, c, a.N, p);
+        load8<float>((const glob<float> *)a.part + ((u64)s * a.M + r) * a.N, c, a.N, p);
 #pragma unroll
         for (u32 j = 0; j < 8; j++) v[j] += p[j];
     }
-    unscale8<PL>(a, r, c, v);
+    if (PL == 2) {
+        int ec[8];
+        const int er = ((const glob<int> *)a.ea)[r];
+        if (column_exps(a, c, ec) || exp_marked(er)) {
+            for (u32 j = 0; j < 8 && c + j < a.N; j++) finish_marked<PL, T>(a, r, c + j);
+            return;
+        }
+#pragma unroll
+        for (u32 j = 0; j < 8; j++) v[j] = ldexpf(v[j], -(er + ec[j]));
+    }
     finish8<T>(a, r, c, v);
 }
 
@@ -351,7 +455,7 @@ __device__ __forceinline__ void gemm_join(const GemmArgs &a) {
 // 8 values, at the scale of their operand, into a packed operand: row r, k =
 // k0 .. k0 + 7 (k0 a multiple of 8).
 template <u32 PL>
-__device__ __forceinline__ void put_packed(f16 *out, u32 KB, u32 r, u32 k0, const float *v) {
+__device__ __forceinline__ void put_packed(glob<f16> *out, u32 KB, u32 r, u32 k0, const float *v) {
     h8 hi, lo;
 #pragma unroll
     for (u32 j = 0; j < 8; j++) {
@@ -360,17 +464,17 @@ __device__ __forceinline__ void put_packed(f16 *out, u32 KB, u32 r, u32 k0, cons
         hi[j] = h;
         lo[j] = l;
     }
-    f16 *at = out + block_at<PL>(r >> 5, k0 >> 4, KB, 0) + ((k0 >> 3) & 1u) * 256u + (r & 31u) * 8u;
-    *(h8 *)at = hi;
-    if (PL == 2) *(h8 *)(at + 512) = lo;
+    glob<f16> *at = out + block_at<PL>(r >> 5, k0 >> 4, KB, 0) + ((k0 >> 3) & 1u) * 256u + (r & 31u) * 8u;
+    *(glob<h8> *)at = hi;
+    if (PL == 2) *(glob<h8> *)(at + 512) = lo;
 }
 
 template <u32 PL>
-__device__ __forceinline__ void get_packed(const f16 *in, u32 KB, u32 r, u32 k0, float *v) {
-    const f16 *at = in + block_at<PL>(r >> 5, k0 >> 4, KB, 0) + ((k0 >> 3) & 1u) * 256u + (r & 31u) * 8u;
-    const h8 hi = *(const h8 *)at;
+__device__ __forceinline__ void get_packed(const glob<f16> *in, u32 KB, u32 r, u32 k0, float *v) {
+    const glob<f16> *at = in + block_at<PL>(r >> 5, k0 >> 4, KB, 0) + ((k0 >> 3) & 1u) * 256u + (r & 31u) * 8u;
+    const h8 hi = *(const glob<h8> *)at;
     h8 lo = {};
-    if (PL == 2) lo = *(const h8 *)(at + 512);
+    if (PL == 2) lo = *(const glob<h8> *)(at + 512);
 #pragma unroll
     for (u32 j = 0; j < 8; j++) v[j] = PL == 2 ? (float)hi[j] + (float)lo[j] : (float)hi[j];
 }
@@ -389,24 +493,17 @@ __device__ __forceinline__ void ns_tile(const NsArgs &a, f16 *lds) {
     if (a.sym) tile_upper(blockIdx.x, ti, tj);
     else tile_of(blockIdx.x, a.tm, a.tn, ti, tj);
     f16v acc[TL::MI][TL::NI];
-    mainloop<TL>(lds, (const f16 *)(a.A + z * a.stride), (const f16 *)(a.B + z * a.stride), a.KB, a.KB, ti * TL::RBA, tj * TL::RBB,
-                 0, a.KU / TL::KS, acc);
-    wait_stage<0>();
+    mainloop<TL>(lds, (const glob<f16> *)(a.A + z * a.stride), (const glob<f16> *)(a.B + z * a.stride), a.KB, a.KB, ti * TL::RBA, tj * TL::RBB,
+                 0, a.KU / TL::US, acc);
+    wait_stage<0, 0>();
     float *st = (float *)lds + wave * 32 * TL::PITCH;
-    const f16 *old = (const f16 *)(a.old + z * a.stride);
-    f16 *out = (f16 *)(a.out + z * a.stride), *out_t = (f16 *)(a.out_t + z * a.stride);
+    const glob<f16> *old = (const glob<f16> *)(a.old + z * a.stride);
+    glob<f16> *out = (glob<f16> *)(a.out + z * a.stride), *out_t = (glob<f16> *)(a.out_t + z * a.stride);
     const bool mirror = a.out_t && !(a.sym && ti == tj);
 #pragma unroll
     for (u32 i = 0; i < TL::MI; i++) {
         const u32 r0 = ti * TL::TM + ((wave / TL::WN) * TL::MI + i) * 32, c0 = tj * TL::TN + (wave % TL::WN) * TL::NI * 32;
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (u32 j = 0; j < TL::NI; j++)
-#pragma unroll
-            for (u32 v = 0; v < 16; v++)
-                st[((v >> 2) * 8 + (lane >> 5) * 4 + (v & 3)) * TL::PITCH + j * 32 + (lane & 31u)] = acc[i][j][v];
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+        stage_rows<TL>(st, acc[i]);
         // own orientation: lane takes row lane % 32, 8 columns at a time
 #pragma unroll
         for (u32 j = 0; j < TL::NI * 2; j++) {
@@ -445,7 +542,7 @@ __device__ __forceinline__ void ns_tile(const NsArgs &a, f16 *lds) {
         }
         if (a.last) {
             // X is [n][w]; the parameter is X's shape, or its transpose (a.tall)
-            T *p = (T *)a.param[z];
+            glob<T> *p = (glob<T> *)a.param[z];
             float v[8], o[8];
             if (!a.tall) {
                 constexpr u32 LPR = TL::NI * 4, RPP = 64 / LPR;
@@ -455,7 +552,7 @@ __device__ __forceinline__ void ns_tile(const NsArgs &a, f16 *lds) {
                     if (r0 + r >= a.n || c0 + c >= a.w) continue;
                     *(f4 *)v = *(const f4 *)(st + r * TL::PITCH + c);
                     *(f4 *)(v + 4) = *(const f4 *)(st + r * TL::PITCH + c + 4);
-                    T *row = p + (u64)(r0 + r) * a.w;
+                    glob<T> *row = p + (u64)(r0 + r) * a.w;
                     load8<T>(row, c0 + c, a.w, o);
 #pragma unroll
                     for (u32 t = 0; t < 8; t++) o[t] = a.keep * o[t] - a.step * v[t];
@@ -468,7 +565,7 @@ __device__ __forceinline__ void ns_tile(const NsArgs &a, f16 *lds) {
                     if (r0 + r >= a.n || c0 + c >= a.w) continue;
 #pragma unroll
                     for (u32 t = 0; t < 8; t++) v[t] = st[(r + t) * TL::PITCH + c];
-                    T *row = p + (u64)(c0 + c) * a.n;
+                    glob<T> *row = p + (u64)(c0 + c) * a.n;
                     load8<T>(row, r0 + r, a.n, o);
 #pragma unroll
                     for (u32 t = 0; t < 8; t++) o[t] = a.keep * o[t] - a.step * v[t];
@@ -486,16 +583,16 @@ template <typename T>
 __device__ __forceinline__ void muon_momentum(const MuonArgs &a) {
     __shared__ double lds[4];
     const u32 z = blockIdx.y;
-    const T *g = (const T *)a.grad[z];
-    float *m = (float *)a.m[z];
+    const glob<T> *g = (const glob<T> *)a.grad[z];
+    glob<float> *m = (glob<float> *)a.m[z];
     double s = 0.0;
     for (u64 i = ((u64)blockIdx.x * 256u + threadIdx.x) * 4u; i < a.numel; i += (u64)gridDim.x * 1024u) {
         float gv[4], mv[4];
         if (i + 4 <= a.numel) {
-            const Pack<T, 4> pg = *(const Pack<T, 4> *)(g + i);
-            const f4 pm = *(const f4 *)(m + i);
+            const any_vec<T, 4> pg = *(const glob<any_vec<T, 4>> *)(g + i);
+            const f4 pm = *(const glob<f4> *)(m + i);
 #pragma unroll
-            for (u32 j = 0; j < 4; j++) gv[j] = (float)pg.v[j], mv[j] = pm[j];
+            for (u32 j = 0; j < 4; j++) gv[j] = (float)pg[j], mv[j] = pm[j];
         } else {
 #pragma unroll
             for (u32 j = 0; j < 4; j++) gv[j] = i + j < a.numel ? (float)g[i + j] : 0.0f, mv[j] = i + j < a.numel ? m[i + j] : 0.0f;
@@ -507,7 +604,7 @@ __device__ __forceinline__ void muon_momentum(const MuonArgs &a) {
             const double u = a.nesterov ? gv[j] + a.beta * out[j] : out[j];
             s += u * u;
         }
-        if (i + 4 <= a.numel) *(f4 *)(m + i) = out;
+        if (i + 4 <= a.numel) *(glob<f4> *)(m + i) = out;
         else
 #pragma unroll
             for (u32 j = 0; j < 4; j++)
@@ -517,7 +614,7 @@ __device__ __forceinline__ void muon_momentum(const MuonArgs &a) {
     for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
     if ((threadIdx.x & 63u) == 0) lds[threadIdx.x >> 6] = s;
     __syncthreads();
-    if (threadIdx.x == 0) ((double *)a.sums)[z * a.blocks + blockIdx.x] = lds[0] + lds[1] + lds[2] + lds[3];
+    if (threadIdx.x == 0) ((glob<double> *)a.sums)[z * a.blocks + blockIdx.x] = lds[0] + lds[1] + lds[2] + lds[3];
 }
 
 // ---- packing ----
@@ -540,12 +637,11 @@ __device__ __forceinline__ int exp_word(u32 w) {
 // What is packed at (r, c .. c + 7): the matrix itself, or dy * act'(z).
 template <typename T>
 __device__ __forceinline__ void source8(const PackArgs &a, u32 r, u32 c, float *v) {
-    load8<T>((const T *)a.src + (u64)r * a.C, c, a.C, v);
+    load8<T>((const glob<T> *)a.src + (u64)r * a.C, c, a.C, v);
     if (a.z) {
         float z[8];
-        load8<T>((const T *)a.z + (u64)r * a.C, c, a.C, z);
-#pragma unroll
-        for (u32 j = 0; j < 8; j++) v[j] *= act_slope(a.act, z[j]);
+        load8<T>((const glob<T> *)a.z + (u64)r * a.C, c, a.C, z);
+        slope8(a.act, z, v);
     }
 }
 
@@ -578,7 +674,7 @@ __device__ __forceinline__ void pack_sizes(const PackArgs &a) {
         if (a.row_part) {
 #pragma unroll
             for (int d = 32; d; d >>= 1) rw = size_join(rw, __shfl_xor(rw, d));
-            if (lane == 0) ((u32 *)a.row_part)[(u64)blockIdx.x * a.R + r] = rw;
+            if (lane == 0) ((glob<u32> *)a.row_part)[(u64)blockIdx.x * a.R + r] = rw;
         }
     }
     if (!a.col_part && !a.sum_part) return;
@@ -591,8 +687,8 @@ __device__ __forceinline__ void pack_sizes(const PackArgs &a) {
     float s = ls[0][t];
 #pragma unroll
     for (u32 k = 1; k < 8; k++) w = size_join(w, lw[k][t]), s += ls[k][t];
-    if (a.col_part) ((u32 *)a.col_part)[(u64)blockIdx.y * a.C + ct] = w;
-    if (a.sum_part) ((float *)a.sum_part)[(u64)blockIdx.y * a.C + ct] = s;
+    if (a.col_part) ((glob<u32> *)a.col_part)[(u64)blockIdx.y * a.C + ct] = w;
+    if (a.sum_part) ((glob<float> *)a.sum_part)[(u64)blockIdx.y * a.C + ct] = s;
 }
 
 // A 64 x 64 tile of a matrix [R][C] into one or both packed orientations:
@@ -610,9 +706,9 @@ __device__ __forceinline__ void pack_tile(const PackArgs &a, const MuonArgs *mu)
         const u32 i = t >> 2, q = t & 3u;
         u32 wr = 0, wc = 0;
         if (a.pn && r0 + i < a.R)
-            for (u32 p = q; p < a.row_parts; p += 4) wr = size_join(wr, ((const u32 *)a.row_part)[(u64)p * a.R + r0 + i]);
+            for (u32 p = q; p < a.row_parts; p += 4) wr = size_join(wr, ((const glob<u32> *)a.row_part)[(u64)p * a.R + r0 + i]);
         if (a.pt && c0 + i < a.C)
-            for (u32 p = q; p < a.col_parts; p += 4) wc = size_join(wc, ((const u32 *)a.col_part)[(u64)p * a.C + c0 + i]);
+            for (u32 p = q; p < a.col_parts; p += 4) wc = size_join(wc, ((const glob<u32> *)a.col_part)[(u64)p * a.C + c0 + i]);
         wr = size_join(wr, __shfl_xor(wr, 1));
         wc = size_join(wc, __shfl_xor(wc, 1));
         wr = size_join(wr, __shfl_xor(wr, 2));
@@ -620,21 +716,21 @@ __device__ __forceinline__ void pack_tile(const PackArgs &a, const MuonArgs *mu)
         if (q == 0) {
             er[i] = exp_word(wr);
             ec[i] = exp_word(wc);
-            if (a.pn && c0 == 0 && r0 + i < a.Rn) ((int *)a.en)[r0 + i] = er[i];
-            if (a.pt && r0 == 0 && c0 + i < a.Ct) ((int *)a.et)[c0 + i] = ec[i];
+            if (a.pn && c0 == 0 && r0 + i < a.Rn) ((glob<int> *)a.en)[r0 + i] = er[i];
+            if (a.pt && r0 == 0 && c0 + i < a.Ct) ((glob<int> *)a.et)[c0 + i] = ec[i];
         }
     }
     if (MUON) {
         if (t < 64) {
             double s = 0.0;
-            for (u32 i = t; i < mu->blocks; i += 64) s += ((const double *)mu->sums)[zi * mu->blocks + i];
+            for (u32 i = t; i < mu->blocks; i += 64) s += ((const glob<double> *)mu->sums)[zi * mu->blocks + i];
 #pragma unroll
             for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
             if (t == 0) unit_lds = (float)(16384.0 / (sqrt(s) + 1e-7));
         }
     }
     __syncthreads();
-    f16 *pn = (f16 *)(a.pn + zi * a.stride), *pt = (f16 *)(a.pt + zi * a.stride);
+    glob<f16> *pn = (glob<f16> *)(a.pn + zi * a.stride), *pt = (glob<f16> *)(a.pt + zi * a.stride);
 #pragma unroll
     for (u32 h = 0; h < 2; h++) {
         const u32 i = h * 32 + (t >> 3), j = (t & 7u) * 8, r = r0 + i, c = c0 + j;
@@ -642,9 +738,9 @@ __device__ __forceinline__ void pack_tile(const PackArgs &a, const MuonArgs *mu)
         if (r < a.R && c < a.C) {
             if (MUON) {
                 float m[8];
-                load8<float>((const float *)mu->m[zi] + (u64)r * a.C, c, a.C, m);
+                load8<float>((const glob<float> *)mu->m[zi] + (u64)r * a.C, c, a.C, m);
                 if (mu->nesterov) {
-                    load8<T>((const T *)mu->grad[zi] + (u64)r * a.C, c, a.C, v);
+                    load8<T>((const glob<T> *)mu->grad[zi] + (u64)r * a.C, c, a.C, v);
 #pragma unroll
                     for (u32 k = 0; k < 8; k++) v[k] += mu->beta * m[k];
                 } else {
@@ -682,13 +778,13 @@ __device__ __forceinline__ void pack_tile(const PackArgs &a, const MuonArgs *mu)
     if (PL == 1 && a.sum_part && t < 64 && c0 + t < a.C && r0 < a.R) {
         float s = 0.0f;
         for (u32 i = 0; i < 64; i++) s += tile[i][t];
-        ((float *)a.sum_part)[(u64)(r0 / 64u) * a.C + c0 + t] = s;
+        ((glob<float> *)a.sum_part)[(u64)(r0 / 64u) * a.C + c0 + t] = s;
     }
 }
 
 // out[c] = the sum of `parts` rows of [parts][C], 16 waves every 16th part.
 template <typename T>
-__device__ __forceinline__ void sum_parts(const float *part, T *out, u32 C, u32 parts) {
+__device__ __forceinline__ void sum_parts(const glob<float> *part, glob<T> *out, u32 C, u32 parts) {
     __shared__ float lds[16][64];
     const u32 lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = blockIdx.x * 64u + lane;
     float s = 0.0f;
@@ -718,21 +814,21 @@ __device__ __forceinline__ void few_rows(const GemmArgs &a) {
     const u32 kr = wave * 4 + (lane >> 4), c = blockIdx.x * COLS + (lane & 15u) * N;
     const u32 per = a.kper, k0 = blockIdx.y * per, k1 = k0 + per < a.K ? k0 + per : a.K;
     const u32 m0 = blockIdx.z * MR;
-    const T *W = (const T *)a.B, *X = (const T *)a.A + (u64)m0 * a.K;
+    const glob<T> *W = (const glob<T> *)a.B, *X = (const glob<T> *)a.A + (u64)m0 * a.K;
     float acc[MR][N];
 #pragma unroll
     for (u32 r = 0; r < MR; r++)
 #pragma unroll
         for (u32 j = 0; j < N; j++) acc[r][j] = 0.0f;
     for (u32 kb = k0; kb < k1; kb += U * KSTEP) {
-        Pack<T, N> w[U];
+        any_vec<T, N> w[U];
 #pragma unroll
         for (u32 u = 0; u < U; u++) {
             const u32 k = kb + u * KSTEP + kr;
-            if (k < k1 && c + N <= a.N) w[u] = *(const Pack<T, N> *)(W + (u64)k * a.N + c);
+            if (k < k1 && c + N <= a.N) w[u] = *(const glob<any_vec<T, N>> *)(W + (u64)k * a.N + c);
             else
 #pragma unroll
-                for (u32 j = 0; j < N; j++) w[u].v[j] = k < k1 && c + j < a.N ? W[(u64)k * a.N + c + j] : (T)0.0f;
+                for (u32 j = 0; j < N; j++) w[u][j] = k < k1 && c + j < a.N ? W[(u64)k * a.N + c + j] : (T)0.0f;
         }
         __syncthreads();
         for (u32 i = threadIdx.x; i < U * KSTEP * MR; i += 512) {
@@ -747,7 +843,7 @@ __device__ __forceinline__ void few_rows(const GemmArgs &a) {
                 for (u32 r = 0; r < MR; r++) {
                     const float x = xs[u * KSTEP + kr][r];
 #pragma unroll
-                    for (u32 j = 0; j < N; j++) acc[r][j] = fmaf(x, (float)w[u].v[j], acc[r][j]);
+                    for (u32 j = 0; j < N; j++) acc[r][j] = fmaf(x, (float)w[u][j], acc[r][j]);
                 }
     }
     // the 4 lane groups of a wave, then the 8 waves in order, 4 rows at a time
@@ -775,7 +871,7 @@ __device__ __forceinline__ void few_rows(const GemmArgs &a) {
                     for (u32 w = 0; w < 8; w++) s += comb[w][(cc + j) / N][r * N + (cc + j) % N];
                     v[j] = s;
                 }
-                if (a.splits > 1) store8<float>((float *)a.part + ((u64)blockIdx.y * a.M + m0 + rb + r) * a.N, col, a.N, v);
+                if (a.splits > 1) store8<float>((glob<float> *)a.part + ((u64)blockIdx.y * a.M + m0 + rb + r) * a.N, col, a.N, v);
                 else finish8<T>(a, m0 + rb + r, col, v);
             }
         }
@@ -796,12 +892,12 @@ __device__ __forceinline__ void few_rows(const GemmArgs &a) {
         ns_tile<Tile##size##_##name, T>(a, lds);                                                                    \
     }
 #define TILE(...) Tile<__VA_ARGS__>
-GEMM(256, TILE(256, 256, 2, 4, 1, 2), f16, f16)
-GEMM(128, TILE(128, 128, 2, 2, 1, 2), f16, f16)
-GEMM(64, TILE(64, 64, 2, 2, 1, 4), f16, f16)
-GEMM(256, TILE(256, 256, 2, 4, 2, 2), f32, float)
-GEMM(128, TILE(128, 128, 2, 2, 2, 2), f32, float)
-GEMM(64, TILE(64, 64, 2, 2, 2, 4), f32, float)
+GEMM(256, TILE(256, 256, 2, 4, 1, 2, 4), f16, f16)
+GEMM(128, TILE(128, 128, 2, 2, 1, 2, 4), f16, f16)
+GEMM(64, TILE(64, 64, 2, 2, 1, 4, 4), f16, f16)
+GEMM(256, TILE(256, 256, 2, 4, 2, 1, 4), f32, float)
+GEMM(128, TILE(128, 128, 2, 2, 2, 1, 4), f32, float)
+GEMM(64, TILE(64, 64, 2, 2, 2, 2, 4), f32, float)
 
 #define PER_TYPE(PL, name, T)                                                                                      \
     extern "C" __global__ __launch_bounds__(256) void thvm_gemm_join_##name(GemmArgs a) { gemm_join<PL, T>(a); }    \
@@ -813,7 +909,7 @@ GEMM(64, TILE(64, 64, 2, 2, 2, 4), f32, float)
     }                                                                                                              \
     extern "C" __global__ __launch_bounds__(256) void thvm_muon_momentum_##name(MuonArgs m) { muon_momentum<T>(m); } \
     extern "C" __global__ __launch_bounds__(1024) void thvm_sum_parts_##name(u64 part, u64 out, u32 C, u32 parts) { \
-        sum_parts<T>((const float *)part, (T *)out, C, parts);                                                      \
+        sum_parts<T>((const glob<float> *)part, (glob<T> *)out, C, parts);                                                      \
     }                                                                                                              \
     extern "C" __global__ __launch_bounds__(512) void thvm_few1_##name(GemmArgs a) { few_rows<T, 1>(a); }           \
     extern "C" __global__ __launch_bounds__(512) void thvm_few4_##name(GemmArgs a) { few_rows<T, 4>(a); }           \

@@ -94,7 +94,7 @@ typedef struct {
     int no_batch;            /* THVM_HIP_NO_BATCH: launch every dispatch on its own */
     int no_seq;              /* THVM_HIP_NO_SEQ: no sequence kernels for dependent small launches */
     u64 n_stream_sync;       /* host waits on the stream (buf_read, synchronize, ...) */
-    hipModule_t static_mod[3]; /* precompiled kernels */
+    hipModule_t static_mod;  /* precompiled kernels */
     unsigned long long *comb_slots; /* single-pass combines: partial words (cleared after each use) */
     u32 resident_waves;      /* waves the device holds at once for a single-pass grid */
     u32 n_cu;                /* compute units (256 on MI355X; assumed where no device is open) */
@@ -403,7 +403,10 @@ void dense_shutdown(void);
 
 /* ---------------- operators of a residual block (block.c) ---------------- */
 void hipb_operand(u32 id);
-void block_shutdown(void);
+/* its kernels and workspace, with the backend's own; weak: a program that
+ * links the analyses alone leaves block.c out */
+int  block_init(void) __attribute__((weak));
+void block_shutdown(void) __attribute__((weak));
 
 /* ---------------- pooling windows and run sums ---------------- */
 int  window_try_dispatch(u32 out_buf, const u32 *leaf_bufs, u32 n_leaves, const UOpKernel *k);

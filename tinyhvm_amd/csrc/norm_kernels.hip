@@ -13,42 +13,15 @@
 #include <hip/hip_runtime.h>
 #include "thvm_abi.h"
 #include "block_args.h"
-
-typedef _Float16 f16;
+#include "block_mem.h"
 
 template <typename T> struct Vec { static constexpr u32 N = 16 / sizeof(T); };
 
-// A vector that starts at any element: rows of an odd length are aligned to
-// their elements only, which the global loads and stores allow.
-template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Pack { T v[Vec<T>::N]; };
-
-// elements [e, e + N) of a row of `cols`, zeros past its end
-template <typename T>
-__device__ __forceinline__ void load_vec(const T *row, u32 e, u32 cols, float *out) {
-    constexpr u32 N = Vec<T>::N;
-    if (e + N <= cols) {
-        const Pack<T> p = *(const Pack<T> *)(row + e);
-#pragma unroll
-        for (u32 j = 0; j < N; j++) out[j] = (float)p.v[j];
-    } else {
-#pragma unroll
-        for (u32 j = 0; j < N; j++) out[j] = e + j < cols ? (float)row[e + j] : 0.0f;
-    }
+template <typename T> __device__ __forceinline__ void load_vec(const glob<T> *row, u32 e, u32 cols, float *out) {
+    load_n<T, Vec<T>::N>(row, e, cols, out);
 }
-
-template <typename T>
-__device__ __forceinline__ void store_vec(T *row, u32 e, u32 cols, const float *in) {
-    constexpr u32 N = Vec<T>::N;
-    if (e + N <= cols) {
-        Pack<T> p;
-#pragma unroll
-        for (u32 j = 0; j < N; j++) p.v[j] = (T)in[j];
-        *(Pack<T> *)(row + e) = p;
-    } else {
-#pragma unroll
-        for (u32 j = 0; j < N; j++)
-            if (e + j < cols) row[e + j] = (T)in[j];
-    }
+template <typename T> __device__ __forceinline__ void store_vec(glob<T> *row, u32 e, u32 cols, const float *in) {
+    store_n<T, Vec<T>::N>(row, e, cols, in);
 }
 
 __device__ __forceinline__ float wave_sum(float v) {
@@ -88,7 +61,7 @@ __device__ __forceinline__ void ln_fwd(const LnArgs &a) {
     const u32 lane = threadIdx.x % G;
     const u32 r = blockIdx.x * PER + threadIdx.x / G;
     if (PER > 1 && r >= a.rows) return;      // whole waves of their own, no barrier below
-    const T *x = (const T *)a.x + (u64)r * a.cols;
+    const glob<T> *x = (const glob<T> *)a.x + (u64)r * a.cols;
     float v[NV][N];
     float s[1] = {0.0f};
 #pragma unroll
@@ -109,14 +82,14 @@ __device__ __forceinline__ void ln_fwd(const LnArgs &a) {
         }
     group_sum<G, 1>(s, lds, 1);
     const float rstd = 1.0f / sqrtf(s[0] / n + a.eps);
-    T *y = (T *)a.y + (u64)r * a.cols;
+    glob<T> *y = (glob<T> *)a.y + (u64)r * a.cols;
 #pragma unroll
     for (u32 i = 0; i < NV; i++) {
         const u32 e = (lane + i * G) * N;
         if (e >= a.cols) continue;
         float g[N], b[N], o[N];
-        if (a.gamma) load_vec<T>((const T *)a.gamma, e, a.cols, g);
-        if (a.beta) load_vec<T>((const T *)a.beta, e, a.cols, b);
+        if (a.gamma) load_vec<T>((const glob<T> *)a.gamma, e, a.cols, g);
+        if (a.beta) load_vec<T>((const glob<T> *)a.beta, e, a.cols, b);
 #pragma unroll
         for (u32 j = 0; j < N; j++) {
             o[j] = v[i][j] * rstd;
@@ -126,8 +99,8 @@ __device__ __forceinline__ void ln_fwd(const LnArgs &a) {
         store_vec<T>(y, e, a.cols, o);
     }
     if (lane == 0) {
-        if (a.mean) ((float *)a.mean)[r] = mean;
-        if (a.rstd) ((float *)a.rstd)[r] = rstd;
+        if (a.mean) ((glob<float> *)a.mean)[r] = mean;
+        if (a.rstd) ((glob<float> *)a.rstd)[r] = rstd;
     }
 }
 
@@ -137,7 +110,7 @@ __device__ __forceinline__ void ln_fwd_long(const LnArgs &a) {
     constexpr u32 N = Vec<T>::N, G = 1024;
     __shared__ float lds[4][16];
     const u32 r = blockIdx.x;
-    const T *x = (const T *)a.x + (u64)r * a.cols;
+    const glob<T> *x = (const glob<T> *)a.x + (u64)r * a.cols;
     float s[1] = {0.0f}, v[N];
     for (u64 e = (u64)threadIdx.x * N; e < a.cols; e += G * N) {
         load_vec<T>(x, (u32)e, a.cols, v);
@@ -155,12 +128,12 @@ __device__ __forceinline__ void ln_fwd_long(const LnArgs &a) {
     }
     group_sum<G, 1>(s, lds, 1);
     const float rstd = 1.0f / sqrtf(s[0] / n + a.eps);
-    T *y = (T *)a.y + (u64)r * a.cols;
+    glob<T> *y = (glob<T> *)a.y + (u64)r * a.cols;
     for (u64 e = (u64)threadIdx.x * N; e < a.cols; e += G * N) {
         float g[N], b[N];
         load_vec<T>(x, (u32)e, a.cols, v);
-        if (a.gamma) load_vec<T>((const T *)a.gamma, (u32)e, a.cols, g);
-        if (a.beta) load_vec<T>((const T *)a.beta, (u32)e, a.cols, b);
+        if (a.gamma) load_vec<T>((const glob<T> *)a.gamma, (u32)e, a.cols, g);
+        if (a.beta) load_vec<T>((const glob<T> *)a.beta, (u32)e, a.cols, b);
 #pragma unroll
         for (u32 j = 0; j < N; j++) {
             v[j] = (v[j] - mean) * rstd;
@@ -170,8 +143,8 @@ __device__ __forceinline__ void ln_fwd_long(const LnArgs &a) {
         store_vec<T>(y, (u32)e, a.cols, v);
     }
     if (threadIdx.x == 0) {
-        if (a.mean) ((float *)a.mean)[r] = mean;
-        if (a.rstd) ((float *)a.rstd)[r] = rstd;
+        if (a.mean) ((glob<float> *)a.mean)[r] = mean;
+        if (a.rstd) ((glob<float> *)a.rstd)[r] = rstd;
     }
 }
 
@@ -198,24 +171,24 @@ __device__ __forceinline__ void ln_bwd(const LnGradArgs &a) {
     for (u32 i = 0; i < NV; i++) {
 #pragma unroll
         for (u32 j = 0; j < N; j++) dg[i][j] = db[i][j] = 0.0f, gm[i][j] = 1.0f;
-        if (a.gamma) load_vec<T>((const T *)a.gamma, (lane + i * G) * N, a.cols, gm[i]);
+        if (a.gamma) load_vec<T>((const glob<T> *)a.gamma, (lane + i * G) * N, a.cols, gm[i]);
     }
     float y1[NV][N], x1[NV][N];
     u64 r = (u64)blockIdx.x * PER + group;
     if (AHEAD && r < a.rows)
 #pragma unroll
         for (u32 i = 0; i < NV; i++) {
-            load_vec<T>((const T *)a.dy + r * a.cols, (lane + i * G) * N, a.cols, y1[i]);
-            load_vec<T>((const T *)a.x + r * a.cols, (lane + i * G) * N, a.cols, x1[i]);
+            load_vec<T>((const glob<T> *)a.dy + r * a.cols, (lane + i * G) * N, a.cols, y1[i]);
+            load_vec<T>((const glob<T> *)a.x + r * a.cols, (lane + i * G) * N, a.cols, x1[i]);
         }
     for (u32 slot = 0; r < a.rows; r += step, slot ^= 1u) {
         float y[NV][N], xh[NV][N];
-        const float mean = ((const float *)a.mean)[r], rstd = ((const float *)a.rstd)[r];
+        const float mean = ((const glob<float> *)a.mean)[r], rstd = ((const glob<float> *)a.rstd)[r];
         if (!AHEAD)
 #pragma unroll
             for (u32 i = 0; i < NV; i++) {
-                load_vec<T>((const T *)a.dy + r * a.cols, (lane + i * G) * N, a.cols, y1[i]);
-                load_vec<T>((const T *)a.x + r * a.cols, (lane + i * G) * N, a.cols, x1[i]);
+                load_vec<T>((const glob<T> *)a.dy + r * a.cols, (lane + i * G) * N, a.cols, y1[i]);
+                load_vec<T>((const glob<T> *)a.x + r * a.cols, (lane + i * G) * N, a.cols, x1[i]);
             }
 #pragma unroll
         for (u32 i = 0; i < NV; i++)
@@ -224,8 +197,8 @@ __device__ __forceinline__ void ln_bwd(const LnGradArgs &a) {
         if (AHEAD && r + step < a.rows)
 #pragma unroll
             for (u32 i = 0; i < NV; i++) {
-                load_vec<T>((const T *)a.dy + (r + step) * a.cols, (lane + i * G) * N, a.cols, y1[i]);
-                load_vec<T>((const T *)a.x + (r + step) * a.cols, (lane + i * G) * N, a.cols, x1[i]);
+                load_vec<T>((const glob<T> *)a.dy + (r + step) * a.cols, (lane + i * G) * N, a.cols, y1[i]);
+                load_vec<T>((const glob<T> *)a.x + (r + step) * a.cols, (lane + i * G) * N, a.cols, x1[i]);
             }
         // past the row's end dy is 0: nothing there reaches a sum
         float s[2] = {0.0f, 0.0f};
@@ -248,17 +221,17 @@ __device__ __forceinline__ void ln_bwd(const LnGradArgs &a) {
             const u32 e = (lane + i * G) * N;
             if (e >= a.cols) continue;
             float o[N], ad[N];
-            if (a.add) load_vec<T>((const T *)a.add + r * a.cols, e, a.cols, ad);
+            if (a.add) load_vec<T>((const glob<T> *)a.add + r * a.cols, e, a.cols, ad);
 #pragma unroll
             for (u32 j = 0; j < N; j++) {
                 o[j] = rstd * (y[i][j] - c0 - xh[i][j] * c1);
                 if (a.add) o[j] += ad[j];
             }
-            store_vec<T>((T *)a.dx + r * a.cols, e, a.cols, o);
+            store_vec<T>((glob<T> *)a.dx + r * a.cols, e, a.cols, o);
         }
     }
     if (!a.part) return;
-    float *pg = (float *)a.part + (u64)blockIdx.x * 2u * a.cols, *pb = pg + a.cols;
+    glob<float> *pg = (glob<float> *)a.part + (u64)blockIdx.x * 2u * a.cols, *pb = pg + a.cols;
 #pragma unroll
     for (u32 i = 0; i < NV; i++) {
         const u32 e = (lane + i * G) * N;
@@ -291,13 +264,13 @@ __device__ __forceinline__ void ln_bwd_long(const LnGradArgs &a) {
     constexpr u32 N = Vec<T>::N, G = 1024;
     __shared__ float lds[4][16];
     const u64 r = blockIdx.x;
-    const T *x = (const T *)a.x + r * a.cols, *dy = (const T *)a.dy + r * a.cols;
-    const float mean = ((const float *)a.mean)[r], rstd = ((const float *)a.rstd)[r], inv = 1.0f / (float)a.cols;
+    const glob<T> *x = (const glob<T> *)a.x + r * a.cols, *dy = (const glob<T> *)a.dy + r * a.cols;
+    const float mean = ((const glob<float> *)a.mean)[r], rstd = ((const glob<float> *)a.rstd)[r], inv = 1.0f / (float)a.cols;
     float s[2] = {0.0f, 0.0f}, v[N], y[N], g[N];
     for (u64 e = (u64)threadIdx.x * N; e < a.cols; e += G * N) {
         load_vec<T>(x, (u32)e, a.cols, v);
         load_vec<T>(dy, (u32)e, a.cols, y);
-        if (a.gamma) load_vec<T>((const T *)a.gamma, (u32)e, a.cols, g);
+        if (a.gamma) load_vec<T>((const glob<T> *)a.gamma, (u32)e, a.cols, g);
 #pragma unroll
         for (u32 j = 0; j < N; j++) {
             if (e + j >= a.cols) continue;
@@ -312,15 +285,15 @@ __device__ __forceinline__ void ln_bwd_long(const LnGradArgs &a) {
         float ad[N];
         load_vec<T>(x, (u32)e, a.cols, v);
         load_vec<T>(dy, (u32)e, a.cols, y);
-        if (a.gamma) load_vec<T>((const T *)a.gamma, (u32)e, a.cols, g);
-        if (a.add) load_vec<T>((const T *)a.add + r * a.cols, (u32)e, a.cols, ad);
+        if (a.gamma) load_vec<T>((const glob<T> *)a.gamma, (u32)e, a.cols, g);
+        if (a.add) load_vec<T>((const glob<T> *)a.add + r * a.cols, (u32)e, a.cols, ad);
 #pragma unroll
         for (u32 j = 0; j < N; j++) {
             const float t = a.gamma ? y[j] * g[j] : y[j];
             v[j] = rstd * (t - c0 - (v[j] - mean) * rstd * c1);
             if (a.add) v[j] += ad[j];
         }
-        store_vec<T>((T *)a.dx + r * a.cols, (u32)e, a.cols, v);
+        store_vec<T>((glob<T> *)a.dx + r * a.cols, (u32)e, a.cols, v);
     }
 }
 
@@ -334,11 +307,11 @@ __device__ __forceinline__ void ln_part_long(const LnGradArgs &a) {
     const u64 r1 = r0 + per < a.rows ? r0 + per : a.rows;
     float dg = 0.0f, db = 0.0f;
     for (u64 r = r0; r < r1; r++) {
-        const float y = (float)((const T *)a.dy)[r * a.cols + c];
-        dg += y * (((float)((const T *)a.x)[r * a.cols + c] - ((const float *)a.mean)[r]) * ((const float *)a.rstd)[r]);
+        const float y = (float)((const glob<T> *)a.dy)[r * a.cols + c];
+        dg += y * (((float)((const glob<T> *)a.x)[r * a.cols + c] - ((const glob<float> *)a.mean)[r]) * ((const glob<float> *)a.rstd)[r]);
         db += y;
     }
-    float *p = (float *)a.part + (u64)blockIdx.y * 2u * a.cols;
+    glob<float> *p = (glob<float> *)a.part + (u64)blockIdx.y * 2u * a.cols;
     p[c] = dg;
     p[a.cols + c] = db;
 }
@@ -353,13 +326,13 @@ __device__ __forceinline__ void ln_cols(const LnGradArgs &a) {
     const u64 c = (u64)blockIdx.x * 64u + lane, n2 = 2ull * a.cols;
     float s = 0.0f;
     if (c < n2)
-        for (u32 p = wave; p < a.parts; p += 16) s += ((const float *)a.part)[p * n2 + c];
+        for (u32 p = wave; p < a.parts; p += 16) s += ((const glob<float> *)a.part)[p * n2 + c];
     lds[wave][lane] = s;
     __syncthreads();
     if (wave || c >= n2) return;
 #pragma unroll
     for (u32 w = 1; w < 16; w++) s += lds[w][lane];
-    T *out = c < a.cols ? (T *)a.dgamma : (T *)a.dbeta;
+    glob<T> *out = c < a.cols ? (glob<T> *)a.dgamma : (glob<T> *)a.dbeta;
     if (out) out[c < a.cols ? c : c - a.cols] = (T)s;
 }
 

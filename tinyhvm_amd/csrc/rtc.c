@@ -19,14 +19,13 @@
 
 #include "hipb.h"
 
-extern const unsigned char thvm_static_kernels_co[], thvm_norm_kernels_co[], thvm_gemm_kernels_co[];
+extern const unsigned char thvm_static_kernels_co[];
+extern const unsigned long thvm_static_kernels_co_len;
 
-#define STATIC_FNS 512 /* more than the precompiled modules have kernels */
 static struct {
     KCacheEntry *tab;
     u32 cap, n;
     int static_loaded;
-    struct { char name[48]; hipFunction_t fn; } fn[STATIC_FNS];
 } R;
 
 static const char *RTC_OPTS[] = {
@@ -89,14 +88,13 @@ int rtc_init(void) {
     R.n = 0;
     R.tab = calloc(R.cap, sizeof(KCacheEntry));
     if (!R.tab) return -1;
-    const unsigned char *co[] = {thvm_static_kernels_co, thvm_norm_kernels_co, thvm_gemm_kernels_co};
-    for (R.static_loaded = 0; R.static_loaded < 3; R.static_loaded++) {
-        hipError_t e = hipModuleLoadData(&hipb.static_mod[R.static_loaded], co[R.static_loaded]);
-        if (e != hipSuccess) {
-            fprintf(stderr, "tinyhvm-hip: loading a static kernel module failed: %s\n", hipGetErrorString(e));
-            return -1;
-        }
+    hipError_t e = hipModuleLoadData(&hipb.static_mod, thvm_static_kernels_co);
+    if (e != hipSuccess) {
+        fprintf(stderr, "tinyhvm-hip: loading the static kernel module failed: %s\n",
+                hipGetErrorString(e));
+        return -1;
     }
+    R.static_loaded = 1;
     return 0;
 }
 
@@ -113,32 +111,18 @@ void rtc_shutdown(void) {
         }
         free(R.tab);
     }
-    for (int i = 0; i < R.static_loaded; i++) HIPB_CHECK(hipModuleUnload(hipb.static_mod[i]));
+    if (R.static_loaded) HIPB_CHECK(hipModuleUnload(hipb.static_mod));
     memset(&R, 0, sizeof(R));
 }
 
-/* By name, each looked up once: a call has no search to wait for after. */
 hipFunction_t rtc_static_fn(const char *name) {
-    u32 h = 2166136261u;
-    for (const char *c = name; *c; c++) h = (h ^ (u8)*c) * 16777619u;
-    for (u32 p = h % STATIC_FNS, n = 0; n < STATIC_FNS; p = (p + 1) % STATIC_FNS, n++) {
-        if (R.fn[p].name[0] && strcmp(R.fn[p].name, name) != 0) continue;
-        if (R.fn[p].name[0]) return R.fn[p].fn;
-        hipFunction_t f = NULL;
-        for (int i = 0; i < R.static_loaded && !f; i++)
-            if (hipModuleGetFunction(&f, hipb.static_mod[i], name) != hipSuccess) {
-                (void)hipGetLastError(); /* it may be in the next module: no error of this thread's */
-                f = NULL;
-            }
-        if (!f) {
-            fprintf(stderr, "tinyhvm-hip: static kernel %s not found\n", name);
-            return NULL;
-        }
-        snprintf(R.fn[p].name, sizeof R.fn[p].name, "%s", name);
-        R.fn[p].fn = f;
-        return f;
+    hipFunction_t f = NULL;
+    if (!R.static_loaded) return NULL;
+    if (hipModuleGetFunction(&f, hipb.static_mod, name) != hipSuccess) {
+        fprintf(stderr, "tinyhvm-hip: static kernel %s not found\n", name);
+        return NULL;
     }
-    return NULL;
+    return f;
 }
 
 KCacheEntry *rtc_lookup(u64 key, const UOpKernel *k) {
