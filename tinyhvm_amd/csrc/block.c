@@ -8,7 +8,6 @@
  */
 #include <math.h>
 #include <string.h>
-#include <stdlib.h>
 
 #include "hipb.h"
 #include "thvm_hip.h"
@@ -17,10 +16,12 @@
 extern const unsigned char thvm_norm_kernels_co[], thvm_gemm_kernels_co[];
 
 #define MODULES 2
+#define COUNTS 4096u /* outputs of one launch whose sums several workgroups have parts of */
 #define KERNELS 256 /* more than the modules have */
 static struct {
     hipModule_t mod[MODULES];
     struct { char name[48]; hipFunction_t fn; } fn[KERNELS];
+    u64 counts, counts_cap;     /* [COUNTS] u32: 0 between launches */
 } B;
 static Scratch block_ws;
 
@@ -28,6 +29,7 @@ void block_shutdown(void) {
     scratch_release(&block_ws);
     for (int i = 0; i < MODULES; i++)
         if (B.mod[i]) HIPB_CHECK(hipModuleUnload(B.mod[i]));
+    pool_block_put((void *)(uintptr_t)B.counts, B.counts_cap);
     memset(&B, 0, sizeof B);
 }
 
@@ -42,7 +44,13 @@ int block_init(void) {
             return -1;
         }
     }
-    return 0;
+    u32 n = COUNTS, zero = 0;
+    void *counts = pool_block_get(4ull * COUNTS, &B.counts_cap);
+    hipFunction_t fill = rtc_static_fn("thvm_fill_u32");
+    if (!counts || !fill) return -1;
+    B.counts = (u64)(uintptr_t)counts;
+    void *args[] = {&counts, &n, &zero};
+    return hipb_launch(fill, (n + 255) / 256, 1, 1, 256, args) ? 0 : -1;
 }
 
 /* A kernel by name, looked up in the modules once. */
@@ -266,117 +274,176 @@ static void packed_carve(Packed *p, Carve *c, u32 dtype) {
 }
 
 /* A product's tile and K splits: C [M][N] over K. */
-typedef struct { u32 tile, tm, tn, splits; } Plan;
+typedef struct { u32 T, tm, tn, splits, lanes; f32 time; const char *name; } Plan;
 
+/* Tiles, largest first: the larger, the fewer bytes per product, and the fewer
+ * workgroups. What each takes, in us, as measured on products of 512 to 4096
+ * rows and columns over K of 512 to 8192: `unit` per 16 of K (f16, f32; with
+ * every compute unit at work), `fixed` for the launch, the first loads and the
+ * epilogue, `join0 + join1 * splits` for joining K splits. */
+static const struct {
+    u32 T, lanes, slots;      /* slots: workgroups a compute unit holds, which then share its time */
+    const char *name;
+    f32 unit[2], fixed[2], join;
+} TILES[] = {
+    {256, 512, 1, "256x256", {0.41f, 1.15f}, {10, 18}, 15},
+    {128, 256, 1, "128x128", {0.13f, 0.335f}, {6, 9}, 5},
+    {64, 256, 2, "64x64", {0.055f, 0.11f}, {5, 6}, 3},
+};
+
+/* The tile and splits that the estimate puts first. */
 static Plan plan_of(u32 M, u32 N, u32 K, u32 dtype) {
-    static const u32 sizes[] = {256, 128, 64};
-    const u32 cu = hipb.n_cu ? hipb.n_cu : 256;
-    Plan p = {0, 0, 0, 1};
-    for (u32 i = 0; i < 3; i++) {
-        p.tile = sizes[i];
-        p.tm = (u32)div_up(M, p.tile);
-        p.tn = (u32)div_up(N, p.tile);
-        if ((u64)p.tm * p.tn >= cu * 3 / 4) break;
+    const u32 cu = hipb.n_cu ? hipb.n_cu : 256, f = dtype == DTYPE_F32;
+    const f32 units = (f32)(round_up(K, 64) / 16);
+    Plan best;
+    memset(&best, 0, sizeof best);
+    f32 least = 0;
+    for (u32 i = 0; i < sizeof TILES / sizeof TILES[0]; i++) {
+        const u32 tm = (u32)div_up(M, TILES[i].T), tn = (u32)div_up(N, TILES[i].T);
+        const u64 tiles = (u64)tm * tn;
+        for (u32 s = 1; s <= 16; s *= 2) {
+            if (s > 1 && (tiles > COUNTS || units / s < 16)) break;
+            const u64 wgs = tiles * s, rounds = div_up(wgs, (u64)cu * TILES[i].slots);
+            /* two workgroups of a compute unit take 1.9 times one's time */
+            const f32 share = TILES[i].slots == 2 && wgs > cu ? (rounds > 1 ? 1.9f * rounds : 1.9f) : (f32)rounds;
+            const f32 t = TILES[i].fixed[f] + share * units / s * TILES[i].unit[f] + (s > 1 ? TILES[i].join + s + (f32)wgs * TILES[i].T * TILES[i].T * 4 / 3e6f : 0);
+            if (best.T && t >= least) continue;
+            least = t;
+            best = (Plan){TILES[i].T, tm, tn, s, TILES[i].lanes, t, TILES[i].name};
+        }
     }
-    /* workgroups that the card holds at once: LDS is one 256 tile's, or two of the others' */
-    const u64 tiles = (u64)p.tm * p.tn, slots = p.tile == 256 ? cu : 2 * cu, chunks = round_up(K, 64) / 64;
-    while (tiles * p.splits * 2 <= slots && chunks / (p.splits * 2) >= 4 && p.splits < 16) p.splits *= 2;
-    if (getenv("PLANX")) { int t, sp; sscanf(getenv("PLANX"), "%d,%d", &t, &sp); p.tile = t; p.tm = div_up(M, t); p.tn = div_up(N, t); p.splits = sp; }
-    return p;
+    return best;
 }
 
-static u64 plan_part_bytes(const Plan *p, u32 M, u32 N) { return p->splits > 1 ? 4ull * p->splits * M * N : 0; }
+static u64 plan_part_bytes(const Plan *p) { return p->splits > 1 ? 4ull * p->tm * p->tn * p->splits * p->T * p->T : 0; }
 
 /* The product of two packed operands with its epilogue (a: out, z, bias, res, act). */
-static int product(const Plan *pl, const Packed *A, const Packed *B, u32 M, u32 N, u32 dtype, u64 part, GemmArgs a) {
+static int product(const Plan *pl, const Packed *pa, const Packed *pb, u32 M, u32 N, u32 dtype, u64 part, GemmArgs a) {
     char name[48];
-    a.A = A->p; a.B = B->p; a.ea = A->e; a.eb = B->e;
-    a.M = M; a.N = N; a.KB = A->KB;
-    a.tm = pl->tm; a.tn = pl->tn; a.splits = pl->splits; a.part = part;
-    snprintf(name, sizeof name, "thvm_gemm_%u_%s", pl->tile, tname(dtype));
-    int rc = launch1(name, (u64)pl->tm * pl->tn, pl->splits, 1, pl->tile == 256 ? 512 : 256, &a);
-    if (rc || pl->splits == 1) return rc;
-    snprintf(name, sizeof name, "thvm_gemm_join_%s", tname(dtype));
-    return launch1(name, div_up(div_up(N, 8) * M, 256), 1, 1, 256, &a);
+    a.A = pa->p; a.B = pb->p; a.ea = pa->e; a.eb = pb->e;
+    a.M = M; a.N = N; a.KB = pa->KB;
+    a.tm = pl->tm; a.tn = pl->tn; a.splits = pl->splits;
+    a.part = part; a.count = B.counts;
+    snprintf(name, sizeof name, "thvm_gemm_%s_%s", pl->name, tname(dtype));
+    return launch1(name, (u64)pl->tm * pl->tn, pl->splits, 1, pl->lanes, &a);
 }
 
-/* Packing of a matrix [R][C] (times act'(z) where z is given): `rows` with
- * its rows as rows, `cols` with its columns, either or both; and the partial
- * column sums. Parts live in the workspace from `parts` on. */
+/* A matrix [R][C] to pack (times act'(z) where z is given): `rows` with its
+ * rows as rows, `cols` with its columns, either or both, and its column sums.
+ * The parts of its sizes and sums lie in the workspace. */
+typedef struct {
+    u64 src, z;
+    u32 act, R, C;
+    const Packed *rows, *cols;
+    u64 sums, row_part, col_part, sum_part;
+    u32 rt, row_parts, col_parts;
+} Source;
+
 #define SIZE_COLS 512u
 #define SIZE_PARTS 64u
-static u64 pack_parts_bytes(u32 R, u32 C, u32 dtype) {
-    if (dtype == DTYPE_F16) return 4ull * div_up(R, 64) * C;
-    return 4ull * div_up(C, SIZE_COLS) * R + 2 * 4ull * SIZE_PARTS * C + 3072;
+static void source_carve(Source *s, Carve *c, u32 dtype) {
+    s->rt = dtype == DTYPE_F16 ? 64 : (u32)(div_up(div_up(s->R, SIZE_PARTS), 32) * 32);
+    if (!s->rt) s->rt = 32;
+    s->row_parts = (u32)div_up(s->C, SIZE_COLS);
+    s->col_parts = (u32)div_up(s->R, s->rt);
+    if (dtype == DTYPE_F32) {
+        s->row_part = carve(c, s->rows ? 4ull * s->row_parts * s->R : 0);
+        s->col_part = carve(c, s->cols ? 4ull * s->col_parts * s->C : 0);
+    }
+    s->sum_part = carve(c, s->sums ? 4ull * s->col_parts * s->C : 0);
 }
 
-static int pack(u64 src, u64 z, u32 act, u32 R, u32 C, u32 dtype, const Packed *rows, const Packed *cols, u64 parts,
-                u64 sums_out) {
+/* Up to three matrices: their sizes in one launch (f32), their packing in another. */
+static int pack(const Source *src, u32 n, u32 dtype) {
     char name[48];
-    PackArgs a;
-    memset(&a, 0, sizeof a);
-    a.src = src; a.z = act ? z : 0; a.act = act; a.R = R; a.C = C;
-    int rc = THVM_HIP_OK;
-    u32 sum_parts = (u32)div_up(R, 64);
-    if (dtype == DTYPE_F32) {
-        Carve c = {0, parts};
-        a.rt = (u32)(div_up(div_up(R, SIZE_PARTS), 8) * 8);
-        if (a.rt < 32) a.rt = 32;
-        a.row_parts = (u32)div_up(C, SIZE_COLS);
-        a.col_parts = sum_parts = (u32)div_up(R, a.rt);
-        if (rows) a.row_part = carve(&c, 4ull * a.row_parts * R);
-        if (cols) a.col_part = carve(&c, 4ull * a.col_parts * C);
-        if (sums_out) a.sum_part = carve(&c, 4ull * a.col_parts * C);
-        snprintf(name, sizeof name, "thvm_pack_sizes_%s", tname(dtype));
-        rc = launch1(name, a.row_parts, a.col_parts, 1, 512, &a);
-    } else if (sums_out) a.sum_part = parts;
-    if (!rc && (rows || cols || dtype == DTYPE_F16)) {
-        PackArgs b = a;
-        if (dtype == DTYPE_F32) b.sum_part = 0;
-        u32 rmax = (u32)round_up(R, 64), cmax = (u32)round_up(C, 64);
-        if (rows) {
-            b.pn = rows->p; b.en = rows->e; b.Rn = rows->Rp; b.KBn = rows->KB;
-            if (rows->Rp > rmax) rmax = rows->Rp;
+    PackSet s, z;
+    memset(&s, 0, sizeof s);
+    memset(&z, 0, sizeof z);
+    u64 tiles = 0, sized = 0;
+    u64 sums = 0;
+    for (u32 i = 0; i < n; i++) {
+        const Source *m = &src[i];
+        PackArgs a;
+        memset(&a, 0, sizeof a);
+        a.src = m->src; a.z = m->act ? m->z : 0; a.act = m->act; a.R = m->R; a.C = m->C;
+        a.rt = m->rt; a.row_parts = m->row_parts; a.col_parts = m->col_parts;
+        a.row_part = m->rows ? m->row_part : 0;
+        a.col_part = m->cols ? m->col_part : 0;
+        a.sum_part = m->sums ? m->sum_part : 0;
+        z.first[i] = (u32)sized;
+        z.p[i] = a;
+        sized += (u64)m->row_parts * m->col_parts;
+        u32 rmax = m->rows || m->cols || dtype == DTYPE_F16 ? (u32)round_up(m->R ? m->R : 1, 64) : 64, cmax = (u32)round_up(m->C ? m->C : 1, 64);
+        if (m->rows) {
+            a.pn = m->rows->p; a.en = m->rows->e; a.Rn = m->rows->Rp; a.KBn = m->rows->KB;
+            if (a.Rn > rmax) rmax = a.Rn;
         }
-        if (cols) {
-            b.pt = cols->p; b.et = cols->e; b.Ct = cols->Rp; b.KBt = cols->KB;
-            if (cols->Rp > cmax) cmax = cols->Rp;
+        if (m->cols) {
+            a.pt = m->cols->p; a.et = m->cols->e; a.Ct = m->cols->Rp; a.KBt = m->cols->KB;
+            if (a.Ct > cmax) cmax = a.Ct;
         }
-        b.ctiles = cmax / 64;
-        /* column sums are written once a row tile of the matrix itself */
-        snprintf(name, sizeof name, "thvm_pack_%s", tname(dtype));
-        rc = launch1(name, (u64)(rmax / 64) * b.ctiles, 1, 1, 256, &b);
-        if (dtype == DTYPE_F16) sum_parts = (u32)div_up(R, 64);
+        a.sum_out = m->sums;
+        if (m->sums) sums = i + 1;
+        a.ctiles = cmax / 64;
+        s.first[i] = (u32)tiles;
+        s.p[i] = a;
+        tiles += (u64)(rmax / 64) * a.ctiles;
     }
-    if (!rc && sums_out) {
-        void *params[] = {&a.sum_part, &sums_out, &C, &sum_parts};
+    s.n = z.n = n;
+    int rc = THVM_HIP_OK;
+    if (dtype == DTYPE_F32) {
+        snprintf(name, sizeof name, "thvm_pack_sizes_%s", tname(dtype));
+        rc = launch1(name, sized, 1, 1, 512, &z);
+    }
+    if (!rc) {
+        snprintf(name, sizeof name, "thvm_pack_%s", tname(dtype));
+        rc = launch1(name, tiles, 1, 1, 256, &s);
+    }
+    if (!rc && sums && dtype == DTYPE_F16) {
+        const Source *m = &src[sums - 1];
+        void *params[] = {(void *)&m->sum_part, (void *)&m->sums, (void *)&m->C, (void *)&m->col_parts};
         snprintf(name, sizeof name, "thvm_sum_parts_%s", tname(dtype));
-        rc = launch(name, div_up(C, 64), 1, 1, 1024, params);
+        rc = launch(name, div_up(m->C, 64), 1, 1, 1024, params);
     }
     return rc;
 }
 
-/* Few rows: W is read as it lies (few_rows in gemm_kernels.hip). */
+/* Few rows: W is read as it lies, by blocks of 1, 4 or 16 rows (few_rows in
+ * gemm_kernels.hip). Whether the outputs have counters, or need none. */
+#define FEW_NARROW (4u << 20) /* bytes of W */
+static u32 few_block(u32 m) { return m <= 1 ? 1 : m <= 4 ? 4 : 16; }
+static int few_fits(u32 m, u32 k, u32 n, u32 dtype) {
+    return div_up(n, 256 / esize(dtype)) * div_up(m, few_block(m)) <= COUNTS || k <= FEW_CHUNK;
+}
+
+/* Its time in us, roughly: W's bytes once a block of rows. */
+static f32 few_time(u32 m, u32 k, u32 n, u32 dtype) {
+    return (f32)(8 + (double)k * n * esize(dtype) * div_up(m, few_block(m)) / 3.5e6);
+}
+
 static int few(u32 m, u32 k, u32 n, u32 dtype, GemmArgs a) {
-    const u32 cols = 16 * (u32)(16 / esize(dtype)), mr = m <= 1 ? 1 : m <= 4 ? 4 : 16;
-    const u64 strips = div_up(n, cols), blocks = div_up(m, mr), chunks = div_up(k ? k : 1, 128);
-    u64 splits = 512 / (strips * blocks);
+    const u32 mr = few_block(m);
+    /* A W that is read in a few us has narrow strips of columns and K whole:
+     * joining splits takes 4 us. A longer one has wide strips and about 512
+     * workgroups, two on each compute unit. */
+    const int narrow = k <= FEW_CHUNK && (u64)k * n * esize(dtype) <= FEW_NARROW;
+    const u32 cols = (narrow ? 64 : 256) / (u32)esize(dtype);
+    const u64 strips = div_up(n, cols), blocks = div_up(m, mr);
+    u64 splits = narrow || !few_fits(m, FEW_CHUNK + 1, n, dtype) ? 1 : 512 / (strips * blocks);
     if (splits < 1) splits = 1;
-    if (splits > chunks) splits = chunks;
-    if (splits > 64) splits = 64;
-    a.kper = (u32)(div_up(chunks, splits) * 128);
-    a.splits = (u32)div_up(k ? k : 1, a.kper);
+    u64 per = round_up(div_up(k ? k : 1, splits), narrow ? 256 : 128);
+    if (per > FEW_CHUNK) per = FEW_CHUNK;
+    a.kper = (u32)per;
+    a.splits = (u32)div_up(k ? k : 1, per);
     a.M = m; a.N = n; a.K = k;
     Carve c = {0, 0};
-    carve(&c, a.splits > 1 ? 4ull * a.splits * m * n : 0);
+    carve(&c, a.splits > 1 ? 4ull * a.splits * strips * cols * blocks * mr : 0);
     if (!carve_reserve(&c)) return THVM_HIP_ENOMEM;
     a.part = carve(&c, 0);
+    a.count = B.counts;
     char name[48];
-    snprintf(name, sizeof name, "thvm_few%u_%s", mr, tname(dtype));
-    int rc = launch1(name, strips, a.splits, (u32)blocks, 512, &a);
-    if (rc || a.splits == 1) return rc;
-    snprintf(name, sizeof name, "thvm_few_join_%s", tname(dtype));
-    return launch1(name, div_up(div_up(n, 8) * m, 256), 1, 1, 256, &a);
+    snprintf(name, sizeof name, "thvm_few%u%s_%s", mr, narrow ? "n" : "", tname(dtype));
+    return launch1(name, strips, a.splits, (u32)blocks, 512, &a);
 }
 
 int thvm_hip_linear(u32 y, u32 z, u32 x, u32 w, u32 bias, u32 res, u32 act, u32 m, u32 k, u32 n, u32 dtype) {
@@ -394,26 +461,27 @@ int thvm_hip_linear(u32 y, u32 z, u32 x, u32 w, u32 bias, u32 res, u32 act, u32 
     memset(&a, 0, sizeof a);
     a.out = addr(y); a.z = addr(z); a.bias = addr(bias); a.res = addr(res); a.act = act;
     int rc;
-    if (m <= 16 || !k) {
+    const Plan pl = plan_of(m, n, k, dtype);
+    /* packing takes a launch and the operands' bytes twice over (f32: two launches, three times) */
+    const f32 packed = pl.time + (dtype == DTYPE_F16 ? 6 : 12) + (f32)((double)k * (m + (double)n) * 10 / 4e6);
+    if (!k || (few_fits(m, k, n, dtype) && (m <= 16 || (m <= 64 && few_time(m, k, n, dtype) < packed)))) {
         operands_ready(o, 6);
         a.A = addr(x); a.B = addr(w);
         rc = few(m, k, n, dtype, a);
     } else {
-        const Plan pl = plan_of(m, n, k, dtype);
-        Packed px = packed_of(m, k, pl.tile), pw = packed_of(n, k, pl.tile);
-        u64 parts = 0, part = 0;
+        Packed px = packed_of(m, k, pl.T), pw = packed_of(n, k, pl.T);
+        Source src[2] = {{addr(x), 0, 0, m, k, &px, NULL, 0}, {addr(w), 0, 0, k, n, NULL, &pw, 0}};
+        u64 part = 0;
         Carve c = {0, 0};
         for (int pass = 0; pass < 2; pass++) {
             packed_carve(&px, &c, dtype);
             packed_carve(&pw, &c, dtype);
-            u64 b = pack_parts_bytes(m, k, dtype), b2 = pack_parts_bytes(k, n, dtype);
-            parts = carve(&c, dtype == DTYPE_F32 ? (b > b2 ? b : b2) : 0);
-            part = carve(&c, plan_part_bytes(&pl, m, n));
+            for (int i = 0; i < 2; i++) source_carve(&src[i], &c, dtype);
+            part = carve(&c, plan_part_bytes(&pl));
             if (!pass && !carve_reserve(&c)) return THVM_HIP_ENOMEM;
         }
         operands_ready(o, 6);
-        rc = pack(addr(x), 0, 0, m, k, dtype, &px, NULL, parts, 0);
-        if (!rc) rc = pack(addr(w), 0, 0, k, n, dtype, NULL, &pw, parts, 0);
+        rc = pack(src, 2, dtype);
         if (!rc) rc = product(&pl, &px, &pw, m, n, dtype, part, a);
     }
     operands_written(o, 6);
@@ -437,35 +505,33 @@ int thvm_hip_linear_grad(u32 dx, u32 dw, u32 db, u32 dy, u32 z, u32 x, u32 w, u3
     if (!n) dw = db = 0;
     if (!dx && !dw && !db) return THVM_HIP_OK;
     const Plan px_ = plan_of(m, k, n, dtype), pw_ = plan_of(k, n, m, dtype);
-    Packed zr = packed_of(m, n, px_.tile), wr = packed_of(k, n, px_.tile);       /* dx = dz W^T */
-    Packed xc = packed_of(k, m, pw_.tile), zc = packed_of(n, m, pw_.tile);       /* dW = x^T dz */
-    u64 parts = 0, part = 0;
+    Packed zr = packed_of(m, n, px_.T), wr = packed_of(k, n, px_.T);       /* dx = dz W^T */
+    Packed xc = packed_of(k, m, pw_.T), zc = packed_of(n, m, pw_.T);       /* dW = x^T dz */
+    Source src[3] = {{addr(dy), addr(z), act, m, n, dx ? &zr : NULL, dw ? &zc : NULL, addr(db)}};
+    u32 ns = 1;
+    if (dx) src[ns++] = (Source){addr(w), 0, 0, k, n, &wr, NULL, 0};
+    if (dw) src[ns++] = (Source){addr(x), 0, 0, m, k, NULL, &xc, 0};
+    u64 part = 0;
     Carve c = {0, 0};
     for (int pass = 0; pass < 2; pass++) {
         if (dx) packed_carve(&zr, &c, dtype), packed_carve(&wr, &c, dtype);
         if (dw) packed_carve(&xc, &c, dtype), packed_carve(&zc, &c, dtype);
-        u64 b = pack_parts_bytes(m, n, dtype), b2 = dtype == DTYPE_F32 ? pack_parts_bytes(k, n, dtype) : 0;
-        u64 b3 = dtype == DTYPE_F32 ? pack_parts_bytes(m, k, dtype) : 0;
-        if (b2 > b) b = b2;
-        if (b3 > b) b = b3;
-        parts = carve(&c, b);
-        u64 q = dx ? plan_part_bytes(&px_, m, k) : 0, q2 = dw ? plan_part_bytes(&pw_, k, n) : 0;
+        for (u32 i = 0; i < ns; i++) source_carve(&src[i], &c, dtype);
+        u64 q = dx ? plan_part_bytes(&px_) : 0, q2 = dw ? plan_part_bytes(&pw_) : 0;
         part = carve(&c, q > q2 ? q : q2);
         if (!pass && !carve_reserve(&c)) return THVM_HIP_ENOMEM;
     }
     operands_ready(o, 7);
     GemmArgs a;
     memset(&a, 0, sizeof a);
-    int rc = pack(addr(dy), addr(z), act, m, n, dtype, dx ? &zr : NULL, dw ? &zc : NULL, parts, addr(db));
-    if (dx) {
-        if (!rc) rc = pack(addr(w), 0, 0, k, n, dtype, &wr, NULL, parts, 0);
+    int rc = pack(src, ns, dtype);
+    if (dx && !rc) {
         a.out = addr(dx);
-        if (!rc) rc = product(&px_, &zr, &wr, m, k, dtype, part, a);
+        rc = product(&px_, &zr, &wr, m, k, dtype, part, a);
     }
-    if (dw) {
-        if (!rc) rc = pack(addr(x), 0, 0, m, k, dtype, NULL, &xc, parts, 0);
+    if (dw && !rc) {
         a.out = addr(dw);
-        if (!rc) rc = product(&pw_, &xc, &zc, k, n, dtype, part, a);
+        rc = product(&pw_, &xc, &zc, k, n, dtype, part, a);
     }
     operands_written(o, 7);
     return rc;
@@ -524,7 +590,7 @@ static int muon_chunk(const u32 *param, const u32 *grad, const u32 *m, u32 count
     void *pp[] = {&p, &mu};
     snprintf(name, sizeof name, "thvm_muon_pack_%s", tname(dtype));
     rc = launch(name, (u64)(p.Rn / 64) * p.ctiles, count, 1, 256, pp);
-    snprintf(name, sizeof name, "thvm_ns_%u_%s", tile, tname(dtype));
+    snprintf(name, sizeof name, "thvm_ns_%ux%u_%s", tile, tile, tname(dtype));
     const u32 tn = np / tile, tw = wp / tile, lanes = tile == 256 ? 512 : 256, half = tn * (tn + 1) / 2;
     a.stride = stride; a.n = n; a.w = w; a.tall = (u32)tall; a.keep = keep; a.step = step;
     for (u32 s = 0; s < steps && !rc; s++) {

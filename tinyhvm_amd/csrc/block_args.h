@@ -26,17 +26,20 @@ typedef struct {
 enum { ACT_NONE = 0, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU, ACT_COUNT };
 
 /* bytes past a packed operand that a product's last loads may touch */
-#define PACK_SLACK 16384
+#define PACK_SLACK 32768
 
 /* C[M][N] = sum over k of A[r][k] B[c][k], packed operands (gemm_kernels.hip) */
 typedef struct {
     u64 A, B;                  /* packed; KB blocks of 16 k */
     u64 ea, eb;                /* exponent words of A's and B's rows (32-bit operands) */
     u64 out, z, bias, res;     /* row-major [M][N]; bias [N] */
-    u64 part;                  /* [splits][M][N] f32 */
+    u64 part, count;           /* the K splits' sums, and how many of a tile's are there (0 between launches) */
     u32 M, N, KB, tm, tn, splits, act;
     u32 K, kper, pad;          /* few rows: A is x [M][K], B is W [K][N], kper k a split */
 } GemmArgs;
+
+/* few rows: the longest K split of a workgroup, whose part of x it holds in LDS */
+#define FEW_CHUNK 1024
 
 /* packing of a matrix [R][C] (or of dy * act'(z)) */
 typedef struct {
@@ -48,8 +51,15 @@ typedef struct {
     u64 stride;                /* bytes between the matrices of a batch in pn and pt */
     u32 R, C, act, rt;         /* rt: rows of a column part */
     u32 Rn, KBn, Ct, KBt, row_parts, col_parts;
+    u64 sum_out;               /* [C]: the column sums (32-bit operands) */
     u32 ctiles, pad;           /* tiles of 64 columns */
 } PackArgs;
+
+/* up to three matrices of one launch: p[i] from workgroup first[i] on */
+typedef struct {
+    u32 n, first[3];
+    PackArgs p[3];
+} PackSet;
 
 /* the optimiser's matrices of one launch */
 #define MUON_MAX 16

@@ -156,12 +156,15 @@ struct Tile {
     static constexpr u32 EPI = WAVES * 32 * PITCH * 2;      // f16 elements
     static constexpr u32 LDS = NS * STAGE > EPI ? NS * STAGE : EPI;
     static constexpr u32 Q = RB / WAVES, CH = Q * CK;       // row blocks and chunks a wave brings in a stage
-    static constexpr u32 READS = (MI + NI) * CK;            // fragments a wave reads of a stage
+    // fragments a wave reads of a stage, as far as the counter of reads goes
+    static constexpr u32 READS = (MI + NI) * CK < 15 ? (MI + NI) * CK : 15;
     static constexpr u32 TURN = US == 1 ? 2 : 1;            // stages a turn of the main loop
-    static_assert(READS < 16 && RB % WAVES == 0 && (NS & (NS - 1)) == 0 && CK <= 4 && (US == 1 || US % 2 == 0),
+    static_assert(RB % WAVES == 0 && (NS & (NS - 1)) == 0 && CK <= 4 && (US == 1 || US % 2 == 0),
                   "a wave brings whole row blocks; units alternate between two sets of registers");
     static_assert((NS - 1) * CK * 1024 <= PACK_SLACK, "loads past the end");
 };
+
+template <bool v> struct Flag { static constexpr bool value = v; };
 
 // The sums of a tile over stages s0 .. s1 - 1. A unit's fragments are read
 // from LDS while the unit before is multiplied; where that begins a stage,
@@ -191,64 +194,70 @@ __device__ __forceinline__ void mainloop(f16 *lds, const glob<f16> *A, const glo
     // Past the last stage what follows in memory is brought, for no one to
     // read, so that the count of loads in flight stays the same (a packed
     // operand ends PACK_SLACK short of its allocation).
-    auto bring = [&](u32 buf) {
-#pragma unroll
-        for (u32 q = 0; q < Q; q++) {
-            const u32 dst = (u32)(uintptr_t)(lptr)lds + (buf * TL::STAGE + (wave * Q + q) * (TL::CK * 512u)) * 2u;
-#define BRING(c) if (c < TL::CK) __builtin_amdgcn_global_load_lds((gptr)src[q], (lptr)(uintptr_t)dst, 16, c * 1024, 0);
-            BRING(0) BRING(1) BRING(2) BRING(3)
-#undef BRING
-            src[q] += TL::CK * 512u;
+    auto bring = [&](u32 buf, u32 n) {       // the n-th chunk
+        const u32 q = n / TL::CK, dst = (u32)(uintptr_t)(lptr)lds + (buf * TL::STAGE + (wave * Q + q) * (TL::CK * 512u)) * 2u;
+        switch (n % TL::CK) {                // the offset is part of the instruction
+        case 0: __builtin_amdgcn_global_load_lds((gptr)src[q], (lptr)(uintptr_t)dst, 16, 0, 0); break;
+        case 1: __builtin_amdgcn_global_load_lds((gptr)src[q], (lptr)(uintptr_t)dst, 16, 1024, 0); break;
+        case 2: __builtin_amdgcn_global_load_lds((gptr)src[q], (lptr)(uintptr_t)dst, 16, 2048, 0); break;
+        default: __builtin_amdgcn_global_load_lds((gptr)src[q], (lptr)(uintptr_t)dst, 16, 3072, 0); break;
         }
+        if (n % TL::CK == TL::CK - 1) src[q] += TL::CK * 512u;
     };
     h8 a[2][TL::MI][PL], b[2][TL::NI][PL];
-    auto fetch = [&](u32 buf, u32 k, h8 (&fa)[TL::MI][PL], h8 (&fb)[TL::NI][PL]) {
+    // the n-th fragment of unit k of a stage
+    constexpr u32 FRAGS = (TL::MI + TL::NI) * PL;
+    auto fetch = [&](u32 buf, u32 k, u32 n, h8 (&fa)[TL::MI][PL], h8 (&fb)[TL::NI][PL]) {
         const f16 *st = lds + buf * TL::STAGE + lane * 8u;
-#pragma unroll
-        for (u32 p = 0; p < PL; p++) {
-#pragma unroll
-            for (u32 j = 0; j < TL::NI; j++) fb[j][p] = *(const h8 *)(st + ((TL::RBA + wn * TL::NI + j) * TL::CK + k * PL + p) * 512u);
-#pragma unroll
-            for (u32 i = 0; i < TL::MI; i++) fa[i][p] = *(const h8 *)(st + ((wm * TL::MI + i) * TL::CK + k * PL + p) * 512u);
-        }
+        const u32 p = n / (TL::MI + TL::NI), x = n % (TL::MI + TL::NI);
+        if (x < TL::NI) fb[x][p] = *(const h8 *)(st + ((TL::RBA + wn * TL::NI + x) * TL::CK + k * PL + p) * 512u);
+        else fa[x - TL::NI][p] = *(const h8 *)(st + ((wm * TL::MI + x - TL::NI) * TL::CK + k * PL + p) * 512u);
     };
-    auto multiply = [&](const h8 (&fa)[TL::MI][PL], const h8 (&fb)[TL::NI][PL]) {
-#pragma unroll
-        for (u32 t = 0; t < 2 * PL - 1; t++)       // hi hi, then hi lo and lo hi
-#pragma unroll
-            for (u32 i = 0; i < TL::MI; i++)
-#pragma unroll
-                for (u32 j = 0; j < TL::NI; j++)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[i][t >> 1], fb[j][t & 1], acc[i][j], 0, 0, 0);
-    };
-    // One of the next unit's fragments is read after each of the first
-    // multiplications: left alone, the compiler puts the reads last.
-    auto unit = [&](u32 buf, u32 k, const h8 (&fa)[TL::MI][PL], const h8 (&fb)[TL::NI][PL], h8 (&na)[TL::MI][PL],
+    // The products of a unit (hi hi, then hi lo and lo hi), between them the
+    // reads of the next unit's fragments and, where a stage has begun, the
+    // loads of a stage to come. Left alone, the compiler puts the reads last;
+    // loads issued in one go hold the wave up until the address unit has
+    // taken them all, and the matrix unit waits.
+    // The reads come early, for the last one's latency to pass as well.
+    constexpr u32 MFMAS = TL::MI * TL::NI * (2 * PL - 1), RP = FRAGS * 2 > MFMAS ? 2 : 1;
+    auto unit = [&](auto fresh, u32 buf, u32 into, u32 u, const h8 (&fa)[TL::MI][PL], const h8 (&fb)[TL::NI][PL], h8 (&na)[TL::MI][PL],
                     h8 (&nb)[TL::NI][PL]) {
+        constexpr u32 LOADS = decltype(fresh)::value ? TL::CH : 0;
         __builtin_amdgcn_sched_barrier(0);
-        fetch(buf, k, na, nb);
-        multiply(fa, fb);
 #pragma unroll
-        for (u32 i = 0; i < (TL::MI + TL::NI) * PL; i++) {
+        for (u32 m = 0; m < MFMAS; m++) {
+            const u32 t = m / (TL::MI * TL::NI), i = m / TL::NI % TL::MI, j = m % TL::NI;
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[i][t >> 1], fb[j][t & 1], acc[i][j], 0, 0, 0);
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+#pragma unroll
+            for (u32 n = m * RP; n < (m + 1) * RP && n < FRAGS; n++) {
+                fetch(buf, u, n, na, nb);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+#pragma unroll
+            for (u32 n = m * LOADS / MFMAS; n < (m + 1) * LOADS / MFMAS; n++) {
+                bring(into, n);
+                __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+            }
         }
         __builtin_amdgcn_sched_barrier(0);
     };
 #pragma unroll
-    for (u32 i = 0; i + 1 < NS; i++) bring(i);
+    for (u32 i = 0; i + 1 < NS; i++)
+#pragma unroll
+        for (u32 n = 0; n < TL::CH; n++) bring(i, n);
     wait_stage<(NS - 2) * TL::CH, 0>();
-    fetch(0, 0, a[0], b[0]);
+#pragma unroll
+    for (u32 n = 0; n < FRAGS; n++) fetch(0, 0, n, a[0], b[0]);
     for (u32 s = s0, buf = 0; s < s1; s += TL::TURN) {
 #pragma unroll
         for (u32 u = 0; u < TL::US * TL::TURN; u++) {
-            const bool fresh = (u + 1) % TL::US == 0;       // the next unit begins a stage
-            if (fresh) {
+            if ((u + 1) % TL::US == 0) {       // the next unit begins a stage
                 wait_stage<(NS - 3) * TL::CH, TL::READS>();
-                bring((buf + NS - 1) & (NS - 1));
+                const u32 into = (buf + NS - 1) & (NS - 1);
                 buf = (buf + 1) & (NS - 1);
-            }
-            unit(buf, fresh ? 0 : u + 1, a[u & 1], b[u & 1], a[(u + 1) & 1], b[(u + 1) & 1]);
+                unit(Flag<true>{}, buf, into, 0, a[u & 1], b[u & 1], a[(u + 1) & 1], b[(u + 1) & 1]);
+            } else unit(Flag<false>{}, buf, 0, u + 1, a[u & 1], b[u & 1], a[(u + 1) & 1], b[(u + 1) & 1]);
         }
     }
 }
@@ -287,34 +296,20 @@ __device__ __forceinline__ void stage_rows(float *st, const f16v (&acc)[TL::NI])
 
 // What an output becomes: z = sum (+ bias), y = act(z) (+ residual).
 template <typename T>
-__device__ __forceinline__ void finish8(const GemmArgs &a, u32 r, u32 c, float *v) {
-    float t[8];
-    if (a.bias) {
-        load8<T>((const glob<T> *)a.bias, c, a.N, t);
-#pragma unroll
-        for (u32 j = 0; j < 8; j++) v[j] += t[j];
-    }
-    if (a.z) store8<T>((glob<T> *)a.z + (u64)r * a.N, c, a.N, v);
-    act8(a.act, v);
-    if (a.res) {
-        load8<T>((const glob<T> *)a.res + (u64)r * a.N, c, a.N, t);
-#pragma unroll
-        for (u32 j = 0; j < 8; j++) v[j] += t[j];
-    }
-    store8<T>((glob<T> *)a.out + (u64)r * a.N, c, a.N, v);
-}
-
-// One output whose row or column is marked, its sum computed again.
-template <u32 PL, typename T>
-__device__ __forceinline__ void finish_marked(const GemmArgs &a, u32 r, u32 c) {
-    const int e = exp_of(((const glob<int> *)a.ea)[r]) + exp_of(((const glob<int> *)a.eb)[c]);
-    float v = ldexpf(exact_dot<PL>((const glob<f16> *)a.A, (const glob<f16> *)a.B, a.KB, r, c), -e);
+__device__ __forceinline__ void finish1(const GemmArgs &a, u32 r, u32 c, float v) {
     const u64 at = (u64)r * a.N + c;
     if (a.bias) v += (float)((const glob<T> *)a.bias)[c];
     if (a.z) ((glob<T> *)a.z)[at] = (T)v;
     v = act_of(a.act, v);
     if (a.res) v += (float)((const glob<T> *)a.res)[at];
     ((glob<T> *)a.out)[at] = (T)v;
+}
+
+// One output whose row or column is marked, its sum computed again.
+template <u32 PL, typename T>
+__device__ __forceinline__ void finish_marked(const GemmArgs &a, u32 r, u32 c) {
+    const int e = exp_of(((const glob<int> *)a.ea)[r]) + exp_of(((const glob<int> *)a.eb)[c]);
+    finish1<T>(a, r, c, ldexpf(exact_dot<PL>((const glob<f16> *)a.A, (const glob<f16> *)a.B, a.KB, r, c), -e));
 }
 
 // The exponents of 8 columns (padded to whole tiles), and whether one is marked.
@@ -329,8 +324,80 @@ __device__ __forceinline__ bool column_exps(const GemmArgs &a, u32 c, int *ec) {
     return odd;
 }
 
-// A tile of one product, or of one of its K splits (blockIdx.y): the partial
-// sums then go to a.part[split][M][N] and gemm_join ends the work.
+// ---- sums that several workgroups have parts of ----
+//
+// Each writes its part through to memory (sc1: the scope of the whole card,
+// whose L2 caches do not see each other's lines), waits until it is there,
+// and counts itself; the last to come adds all parts, its own at its place,
+// in their order, so the bits do not depend on which one that is. It leaves
+// the count at 0 for the next launch. No workgroup waits for another.
+#define SC1 16
+typedef u32 u4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ void put_part(u64 base, u32 at, f4 v) {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, v), __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, 0x7FFFFFFF, 0x00020000),
+                                           at, 0, SC1);
+}
+__device__ __forceinline__ f4 get_part(u64 base, u32 at) {
+    return __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(
+        __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, 0x7FFFFFFF, 0x00020000), at, 0, SC1));
+}
+
+// Whether this workgroup is the last of n to come.
+__device__ __forceinline__ bool last_of(u64 count, u32 n) {
+    __shared__ u32 before;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        u32 *c = (u32 *)count;
+        before = __hip_atomic_fetch_add(c, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (before == n - 1) __hip_atomic_store(c, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    return before == n - 1;
+}
+
+// A tile's sums over all K splits: part s of tile t lies at (t splits + s)
+// times the tile's size, as the lanes hold it.
+template <typename TL>
+__device__ __forceinline__ bool join_splits(u64 part, u64 count, u32 tile, u32 split, u32 splits, f16v (&acc)[TL::MI][TL::NI]) {
+    constexpr u32 BYTES = TL::TM * TL::TN * 4;
+    const u64 base = part + (u64)tile * splits * BYTES;
+    const u32 lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const u32 at = wave * (TL::MI * TL::NI * 4096u) + lane * 16u;
+#pragma unroll
+    for (u32 i = 0; i < TL::MI; i++)
+#pragma unroll
+        for (u32 j = 0; j < TL::NI; j++)
+#pragma unroll
+            for (u32 q = 0; q < 4; q++)
+                put_part(base + (u64)split * BYTES, at + (i * TL::NI + j) * 4096u + q * 1024u,
+                         f4{acc[i][j][q * 4], acc[i][j][q * 4 + 1], acc[i][j][q * 4 + 2], acc[i][j][q * 4 + 3]});
+    if (!last_of(count + tile * 4ull, splits)) return false;
+#pragma unroll
+    for (u32 i = 0; i < TL::MI; i++) {
+        f16v sum[TL::NI];
+#pragma unroll
+        for (u32 j = 0; j < TL::NI; j++) sum[j] = 0.0f;
+#pragma unroll 2
+        for (u32 s = 0; s < splits; s++) {
+            f4 p[TL::NI][4];
+#pragma unroll
+            for (u32 j = 0; j < TL::NI; j++)
+#pragma unroll
+                for (u32 q = 0; q < 4; q++) p[j][q] = get_part(base + (u64)s * BYTES, at + (i * TL::NI + j) * 4096u + q * 1024u);
+#pragma unroll
+            for (u32 j = 0; j < TL::NI; j++)
+#pragma unroll
+                for (u32 v = 0; v < 16; v++) sum[j][v] += p[j][v >> 2][v & 3];
+        }
+#pragma unroll
+        for (u32 j = 0; j < TL::NI; j++) acc[i][j] = sum[j];
+    }
+    return true;
+}
+
+// A tile of one product, or of one of its K splits (blockIdx.y).
 template <typename TL, typename T>
 __device__ __forceinline__ void gemm_tile(const GemmArgs &a, f16 *lds) {
     const u32 wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -341,6 +408,7 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs &a, f16 *lds) {
     f16v acc[TL::MI][TL::NI];
     mainloop<TL>(lds, (const glob<f16> *)a.A, (const glob<f16> *)a.B, a.KB, a.KB, ti * TL::RBA, tj * TL::RBB, s0, s1, acc);
     wait_stage<0, 0>();
+    if (a.splits > 1 && !join_splits<TL>(a.part, a.count, blockIdx.x, blockIdx.y, a.splits, acc)) return;
     // A lane keeps 8 columns and takes every RPP-th row of them. The residual
     // of a 32-row block is asked for before the block ahead of it is finished.
     constexpr u32 LPR = TL::NI * 4, RPP = 64 / LPR, PASSES = 32 / RPP;
@@ -348,21 +416,6 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs &a, f16 *lds) {
     const u32 r0 = ti * TL::TM + (wave / TL::WN) * TL::MI * 32 + lane / LPR;
     float *st = (float *)lds + wave * 32 * TL::PITCH;
     const float *row = st + (lane / LPR) * TL::PITCH + dc;
-    if (a.splits > 1) {
-#pragma unroll
-        for (u32 i = 0; i < TL::MI; i++) {
-            stage_rows<TL>(st, acc[i]);
-#pragma unroll
-            for (u32 p = 0; p < PASSES; p++) {
-                const u32 r = r0 + i * 32 + p * RPP;
-                float v[8];
-                *(f4 *)v = *(const f4 *)(row + p * RPP * TL::PITCH);
-                *(f4 *)(v + 4) = *(const f4 *)(row + p * RPP * TL::PITCH + 4);
-                if (r < a.M && c < a.N) store8<float>((glob<float> *)a.part + ((u64)blockIdx.y * a.M + r) * a.N, c, a.N, v);
-            }
-        }
-        return;
-    }
     const bool whole = c + 8 <= a.N;
     float bias[8];
     int ec[8];
@@ -424,32 +477,6 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs &a, f16 *lds) {
         }
 }
 
-// The sums of K splits, in split order, and what an output becomes.
-template <u32 PL, typename T>
-__device__ __forceinline__ void gemm_join(const GemmArgs &a) {
-    const u32 per = (a.N + 7) / 8;
-    const u64 t = (u64)blockIdx.x * 256u + threadIdx.x;
-    if (t >= (u64)per * a.M) return;
-    const u32 r = (u32)(t / per), c = (u32)(t % per) * 8;
-    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0}, p[8];
-    for (u32 s = 0; s < a.splits; s++) {
-        load8<float>((const glob<float> *)a.part + ((u64)s * a.M + r) * a.N, c, a.N, p);
-#pragma unroll
-        for (u32 j = 0; j < 8; j++) v[j] += p[j];
-    }
-    if (PL == 2) {
-        int ec[8];
-        const int er = ((const glob<int> *)a.ea)[r];
-        if (column_exps(a, c, ec) || exp_marked(er)) {
-            for (u32 j = 0; j < 8 && c + j < a.N; j++) finish_marked<PL, T>(a, r, c + j);
-            return;
-        }
-#pragma unroll
-        for (u32 j = 0; j < 8; j++) v[j] = ldexpf(v[j], -(er + ec[j]));
-    }
-    finish8<T>(a, r, c, v);
-}
-
 // ---- the Newton-Schulz step's products ----
 
 // 8 values, at the scale of their operand, into a packed operand: row r, k =
@@ -502,7 +529,8 @@ __device__ __forceinline__ void ns_tile(const NsArgs &a, f16 *lds) {
     const bool mirror = a.out_t && !(a.sym && ti == tj);
 #pragma unroll
     for (u32 i = 0; i < TL::MI; i++) {
-        const u32 r0 = ti * TL::TM + ((wave / TL::WN) * TL::MI + i) * 32, c0 = tj * TL::TN + (wave % TL::WN) * TL::NI * 32;
+        const u32 r0 = ti * TL::TM + ((wave / TL::WN) * TL::MI + i) * 32;
+        const u32 c0 = tj * TL::TN + (wave % TL::WN) * TL::NI * 32;
         stage_rows<TL>(st, acc[i]);
         // own orientation: lane takes row lane % 32, 8 columns at a time
 #pragma unroll
@@ -634,6 +662,11 @@ __device__ __forceinline__ int exp_word(u32 w) {
     return w & 0x80000000u ? e ^ EXP_MARK : e;
 }
 
+// The matrix of a set that a workgroup works on.
+__device__ __forceinline__ u32 pack_of(const PackSet &s, u32 block) {
+    return (s.n > 1 && block >= s.first[1]) + (s.n > 2 && block >= s.first[2]);
+}
+
 // What is packed at (r, c .. c + 7): the matrix itself, or dy * act'(z).
 template <typename T>
 __device__ __forceinline__ void source8(const PackArgs &a, u32 r, u32 c, float *v) {
@@ -647,48 +680,54 @@ __device__ __forceinline__ void source8(const PackArgs &a, u32 r, u32 c, float *
 
 // The largest values of a matrix's rows and columns (as size words, a part a
 // column tile of 512 and a row tile of a.rt) and the columns' sums.
-// 8 waves, each every 8th row of the tile, a lane 8 columns.
+// 8 waves, each every 8th row of the tile, a lane 8 columns; four rows are
+// asked for at a time.
 template <typename T>
-__device__ __forceinline__ void pack_sizes(const PackArgs &a) {
+__device__ __forceinline__ void pack_sizes(const PackArgs &a, u32 block) {
     __shared__ u32 lw[8][512];
     __shared__ float ls[8][512];
-    const u32 lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    const u32 c = blockIdx.x * 512u + lane * 8u;
-    const u64 r0 = (u64)blockIdx.y * a.rt, r1 = r0 + a.rt < a.R ? r0 + a.rt : a.R;
+    const u32 lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, bx = block % a.row_parts, by = block / a.row_parts;
+    const u32 c = bx * 512u + lane * 8u;
+    const u64 r0 = (u64)by * a.rt, r1 = r0 + a.rt < a.R ? r0 + a.rt : a.R;
     u32 cw[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     float cs[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    for (u64 r = r0 + wave; r < r1; r += 8) {
-        float v[8];
-        if (c < a.C) source8<T>(a, (u32)r, c, v);
-        else
+    for (u64 r = r0 + wave; r < r1; r += 32) {
+        float v[4][8];
 #pragma unroll
-            for (u32 j = 0; j < 8; j++) v[j] = 0.0f;
-        u32 rw = 0;
+        for (u32 q = 0; q < 4; q++)
+            if (r + q * 8 < r1 && c < a.C) source8<T>(a, (u32)r + q * 8, c, v[q]);
+            else
 #pragma unroll
-        for (u32 j = 0; j < 8; j++) {
-            const u32 w = size_word(v[j]);
-            rw = size_join(rw, w);
-            cw[j] = size_join(cw[j], w);
-            cs[j] += v[j];
-        }
-        if (a.row_part) {
+                for (u32 j = 0; j < 8; j++) v[q][j] = 0.0f;
 #pragma unroll
-            for (int d = 32; d; d >>= 1) rw = size_join(rw, __shfl_xor(rw, d));
-            if (lane == 0) ((glob<u32> *)a.row_part)[(u64)blockIdx.x * a.R + r] = rw;
+        for (u32 q = 0; q < 4; q++) {
+            u32 rw = 0;
+#pragma unroll
+            for (u32 j = 0; j < 8; j++) {
+                const u32 w = size_word(v[q][j]);
+                rw = size_join(rw, w);
+                cw[j] = size_join(cw[j], w);
+                cs[j] += v[q][j];
+            }
+            if (a.row_part && r + q * 8 < r1) {
+#pragma unroll
+                for (int d = 32; d; d >>= 1) rw = size_join(rw, __shfl_xor(rw, d));
+                if (lane == 0) ((glob<u32> *)a.row_part)[(u64)bx * a.R + r + q * 8] = rw;
+            }
         }
     }
     if (!a.col_part && !a.sum_part) return;
 #pragma unroll
     for (u32 j = 0; j < 8; j++) lw[wave][lane * 8 + j] = cw[j], ls[wave][lane * 8 + j] = cs[j];
     __syncthreads();
-    const u32 t = threadIdx.x, ct = blockIdx.x * 512u + t;
+    const u32 t = threadIdx.x, ct = bx * 512u + t;
     if (ct >= a.C) return;
     u32 w = lw[0][t];
     float s = ls[0][t];
 #pragma unroll
     for (u32 k = 1; k < 8; k++) w = size_join(w, lw[k][t]), s += ls[k][t];
-    if (a.col_part) ((glob<u32> *)a.col_part)[(u64)blockIdx.y * a.C + ct] = w;
-    if (a.sum_part) ((glob<float> *)a.sum_part)[(u64)blockIdx.y * a.C + ct] = s;
+    if (a.col_part) ((glob<u32> *)a.col_part)[(u64)by * a.C + ct] = w;
+    if (a.sum_part) ((glob<float> *)a.sum_part)[(u64)by * a.C + ct] = s;
 }
 
 // A 64 x 64 tile of a matrix [R][C] into one or both packed orientations:
@@ -696,11 +735,11 @@ __device__ __forceinline__ void pack_sizes(const PackArgs &a) {
 // exponents of their packed row; `unit` (the optimiser) by one factor.
 // MUON: the source is u (muon_momentum) over its norm.
 template <u32 PL, typename T, bool MUON>
-__device__ __forceinline__ void pack_tile(const PackArgs &a, const MuonArgs *mu) {
+__device__ __forceinline__ void pack_tile(const PackArgs &a, const MuonArgs *mu, u32 block) {
     __shared__ float tile[64][65];
     __shared__ int er[64], ec[64];
     __shared__ float unit_lds;
-    const u32 t = threadIdx.x, r0 = (blockIdx.x / a.ctiles) * 64u, c0 = (blockIdx.x % a.ctiles) * 64u, zi = blockIdx.y;
+    const u32 t = threadIdx.x, r0 = (block / a.ctiles) * 64u, c0 = (block % a.ctiles) * 64u, zi = MUON ? blockIdx.y : 0u;
     if (PL == 2 && !MUON) {
         // the parts of this tile's rows and columns, four lanes to each
         const u32 i = t >> 2, q = t & 3u;
@@ -719,6 +758,12 @@ __device__ __forceinline__ void pack_tile(const PackArgs &a, const MuonArgs *mu)
             if (a.pn && c0 == 0 && r0 + i < a.Rn) ((glob<int> *)a.en)[r0 + i] = er[i];
             if (a.pt && r0 == 0 && c0 + i < a.Ct) ((glob<int> *)a.et)[c0 + i] = ec[i];
         }
+    }
+    if (PL == 2 && !MUON && a.sum_out && r0 == 0 && t < 64 && c0 + t < a.C) {
+        // the column sums, from the parts of pack_sizes
+        float s = 0.0f;
+        for (u32 p = 0; p < a.col_parts; p++) s += ((const glob<float> *)a.sum_part)[(u64)p * a.C + c0 + t];
+        ((glob<T> *)a.sum_out)[c0 + t] = (T)s;
     }
     if (MUON) {
         if (t < 64) {
@@ -800,82 +845,136 @@ __device__ __forceinline__ void sum_parts(const glob<float> *part, glob<T> *out,
 
 // ---- few rows ----
 
-// y = x W, MR rows a workgroup (blockIdx.z): W is read once, as it lies ([K][N] row-major),
-// 16 bytes a lane, 16 lanes along a row and the workgroup's 8 waves 32 rows
-// at a time, and multiplied in 32 bits. Bound by W's bytes, so K is split
-// over workgroups (blockIdx.y) until the card is full; the splits' sums meet
-// in gemm_join.
-template <typename T, u32 MR>
+// y = x W, MR rows a workgroup (blockIdx.z). W is read once, as it lies
+// ([K][N] row-major), BYTES a lane, 16 lanes along a row and the workgroup's
+// 8 waves 32 rows at a time. Bound by W's bytes where W is large: 16 bytes a
+// lane, and K split over workgroups (blockIdx.y) until the card is full. Bound
+// by latency where it is small: 4 bytes a lane, which makes four times the
+// workgroups without a split to join. U of a lane's loads are on their way
+// while U are multiplied; a split's part of x lies in LDS from the start, so
+// that the loop has no barrier.
+//
+// Products are 32-bit ones, of 1 or 4 rows on the vector unit, of 16 on the
+// 32-bit matrix instruction (v_mfma_f32_16x16x4_f32: lane l holds k = l / 16
+// of row, or column, l % 16), one for each of a lane's columns; it adds up
+// the wave's 4 rows of W as well.
+template <typename T, u32 MR, u32 BYTES>
 __device__ __forceinline__ void few_rows(const GemmArgs &a) {
-    constexpr u32 N = 16 / sizeof(T), U = 4, KSTEP = 32, COLS = 16 * N;
-    __shared__ float xs[U * KSTEP][MR];
-    __shared__ float comb[8][16][N * (MR > 4 ? 4 : MR) + 1];
+    constexpr u32 N = BYTES / sizeof(T), U = BYTES == 4 ? 8 : 4, WAVES = 8, KSTEP = WAVES * 4, COLS = 16 * N, OUT = MR * COLS;
+    constexpr u32 PITCH = FEW_CHUNK + 4;     // of 16 rows and 4 k a wave reads 64 banks
+    __shared__ float lds[MR * PITCH > WAVES * OUT ? MR * PITCH : WAVES * OUT];
     const u32 lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     const u32 kr = wave * 4 + (lane >> 4), c = blockIdx.x * COLS + (lane & 15u) * N;
     const u32 per = a.kper, k0 = blockIdx.y * per, k1 = k0 + per < a.K ? k0 + per : a.K;
-    const u32 m0 = blockIdx.z * MR;
+    const u32 m0 = blockIdx.z * MR, rows = a.M - m0 < MR ? a.M - m0 : MR;
     const glob<T> *W = (const glob<T> *)a.B, *X = (const glob<T> *)a.A + (u64)m0 * a.K;
-    float acc[MR][N];
+    constexpr u32 R = MR < 16 ? MR : 4;      // rows of sums a lane holds
+    float acc[N][R];
 #pragma unroll
-    for (u32 r = 0; r < MR; r++)
+    for (u32 j = 0; j < N; j++)
 #pragma unroll
-        for (u32 j = 0; j < N; j++) acc[r][j] = 0.0f;
-    for (u32 kb = k0; kb < k1; kb += U * KSTEP) {
-        any_vec<T, N> w[U];
+        for (u32 r = 0; r < R; r++) acc[j][r] = 0.0f;
+    // past the end W is taken as 0, and x too
+    any_vec<T, N> w[2][U];
+    auto ask = [&](u32 kb, any_vec<T, N> (&v)[U]) {
 #pragma unroll
         for (u32 u = 0; u < U; u++) {
             const u32 k = kb + u * KSTEP + kr;
-            if (k < k1 && c + N <= a.N) w[u] = *(const glob<any_vec<T, N>> *)(W + (u64)k * a.N + c);
+            if (k < k1 && c + N <= a.N) v[u] = *(const glob<any_vec<T, N>> *)(W + (u64)k * a.N + c);
             else
 #pragma unroll
-                for (u32 j = 0; j < N; j++) w[u][j] = k < k1 && c + j < a.N ? W[(u64)k * a.N + c + j] : (T)0.0f;
+                for (u32 j = 0; j < N; j++) v[u][j] = k < k1 && c + j < a.N ? W[(u64)k * a.N + c + j] : (T)0.0f;
         }
-        __syncthreads();
-        for (u32 i = threadIdx.x; i < U * KSTEP * MR; i += 512) {
-            const u32 r = i / (U * KSTEP), k = i % (U * KSTEP);
-            xs[k][r] = m0 + r < a.M && kb + k < k1 ? (float)X[(u64)r * a.K + kb + k] : 0.0f;
-        }
-        __syncthreads();
+    };
+    auto multiply = [&](u32 kb, const any_vec<T, N> (&v)[U]) {
 #pragma unroll
-        for (u32 u = 0; u < U; u++)
-            if (kb + u * KSTEP + kr < k1)     // past the end nothing is multiplied: W there is not a value
+        for (u32 u = 0; u < U; u++) {
+            const float *x = lds + kb - k0 + u * KSTEP + kr;
+            if constexpr (MR == 16) {
+                const float xv = x[(lane & 15u) * PITCH];
 #pragma unroll
-                for (u32 r = 0; r < MR; r++) {
-                    const float x = xs[u * KSTEP + kr][r];
-#pragma unroll
-                    for (u32 j = 0; j < N; j++) acc[r][j] = fmaf(x, (float)w[u][j], acc[r][j]);
+                for (u32 j = 0; j < N; j++) {
+                    f4 t = {acc[j][0], acc[j][1], acc[j][2], acc[j][3]};
+                    t = __builtin_amdgcn_mfma_f32_16x16x4f32(xv, (float)v[u][j], t, 0, 0, 0);
+                    acc[j][0] = t[0], acc[j][1] = t[1], acc[j][2] = t[2], acc[j][3] = t[3];
                 }
+            } else {
+#pragma unroll
+                for (u32 r = 0; r < MR; r++)
+#pragma unroll
+                    for (u32 j = 0; j < N; j++) acc[j][r] = fmaf(x[r * PITCH], (float)v[u][j], acc[j][r]);
+            }
+        }
+    };
+    ask(k0, w[0]);
+#pragma unroll
+    for (u32 r = 0; r < MR; r++)
+        for (u32 k = threadIdx.x; k < per; k += 512) lds[r * PITCH + k] = r < rows && k0 + k < k1 ? (float)X[(u64)r * a.K + k0 + k] : 0.0f;
+    __syncthreads();
+    // per is a multiple of U * KSTEP
+    for (u32 kb = k0; kb < k0 + per; kb += 2 * U * KSTEP) {
+        ask(kb + U * KSTEP, w[1]);
+        multiply(kb, w[0]);
+        if (kb + U * KSTEP >= k0 + per) break;
+        ask(kb + 2 * U * KSTEP, w[0]);
+        multiply(kb + U * KSTEP, w[1]);
     }
-    // the 4 lane groups of a wave, then the 8 waves in order, 4 rows at a time
-    constexpr u32 RB = MR > 4 ? 4 : MR;
+    __syncthreads();
+    // the waves' sums, in order
 #pragma unroll
-    for (u32 rb = 0; rb < MR; rb += RB) {
+    for (u32 r = 0; r < R; r++)
 #pragma unroll
-        for (u32 r = 0; r < RB; r++)
-#pragma unroll
-            for (u32 j = 0; j < N; j++) {
-                float s = acc[rb + r][j];
+        for (u32 j = 0; j < N; j++) {
+            if constexpr (MR == 16) lds[wave * OUT + ((lane >> 4) * 4 + r) * COLS + (lane & 15u) * N + j] = acc[j][r];
+            else {
+                float s = acc[j][r];
                 s += __shfl_xor(s, 16);
                 s += __shfl_xor(s, 32);
-                if (lane < 16) comb[wave][lane][r * N + j] = s;
-            }
-        __syncthreads();
-        for (u32 i = threadIdx.x; i < RB * COLS / 8; i += 512) {
-            const u32 r = i / (COLS / 8), cc = (i % (COLS / 8)) * 8, col = blockIdx.x * COLS + cc;
-            if (m0 + rb + r < a.M && col < a.N) {
-                float v[8];
-#pragma unroll
-                for (u32 j = 0; j < 8; j++) {
-                    float s = 0.0f;
-#pragma unroll
-                    for (u32 w = 0; w < 8; w++) s += comb[w][(cc + j) / N][r * N + (cc + j) % N];
-                    v[j] = s;
-                }
-                if (a.splits > 1) store8<float>((glob<float> *)a.part + ((u64)blockIdx.y * a.M + m0 + rb + r) * a.N, col, a.N, v);
-                else finish8<T>(a, m0 + rb + r, col, v);
+                if (lane < 16) lds[wave * OUT + r * COLS + lane * N + j] = s;
             }
         }
-        __syncthreads();
+    __syncthreads();
+    // a lane's outputs; what they are joined and finished with is asked for at once
+    constexpr u32 PER = (OUT + 511) / 512;
+    const u64 tile = (u64)blockIdx.z * gridDim.x + blockIdx.x, part = a.part + tile * a.splits * (OUT * 4u);
+    float sum[PER], bias[PER], res[PER];
+#pragma unroll
+    for (u32 i = 0; i < PER; i++) {
+        const u32 o = threadIdx.x + i * 512;
+        sum[i] = lds[o % OUT];
+#pragma unroll
+        for (u32 q = 1; q < WAVES; q++) sum[i] += lds[q * OUT + o % OUT];
+        if (a.splits > 1 && o < rows * COLS)
+            __hip_atomic_store((float *)(part + ((u64)blockIdx.y * OUT + o) * 4u), sum[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    if (a.splits > 1 && !last_of(a.count + tile * 4u, a.splits)) return;
+#pragma unroll
+    for (u32 i = 0; i < PER; i++) {
+        const u32 o = threadIdx.x + i * 512, r = m0 + o / COLS, col = blockIdx.x * COLS + o % COLS;
+        if (o >= rows * COLS || col >= a.N) continue;
+        if (a.bias) bias[i] = (float)((const glob<T> *)a.bias)[col];
+        if (a.res) res[i] = (float)((const glob<T> *)a.res)[(u64)r * a.N + col];
+    }
+    if (a.splits > 1) {
+#pragma unroll
+        for (u32 i = 0; i < PER; i++) sum[i] = 0.0f;
+#pragma unroll 16
+        for (u32 p = 0; p < a.splits; p++)
+#pragma unroll
+            for (u32 i = 0; i < PER; i++)      // without a condition, which would part the loads
+                sum[i] += __hip_atomic_load((const float *)(part + ((u64)p * OUT + (threadIdx.x + i * 512) % OUT) * 4u), __ATOMIC_RELAXED,
+                                            __HIP_MEMORY_SCOPE_AGENT);
+    }
+#pragma unroll
+    for (u32 i = 0; i < PER; i++) {
+        const u32 o = threadIdx.x + i * 512, r = m0 + o / COLS, col = blockIdx.x * COLS + o % COLS;
+        if (o >= rows * COLS || col >= a.N) continue;
+        const u64 at = (u64)r * a.N + col;
+        float v = a.bias ? sum[i] + bias[i] : sum[i];
+        if (a.z) ((glob<T> *)a.z)[at] = (T)v;
+        v = act_of(a.act, v);
+        if (a.res) v += res[i];
+        ((glob<T> *)a.out)[at] = (T)v;
     }
 }
 
@@ -886,33 +985,47 @@ __device__ __forceinline__ void few_rows(const GemmArgs &a) {
     extern "C" __global__ __launch_bounds__(Tile##size##_##name::THREADS) void thvm_gemm_##size##_##name(GemmArgs a) { \
         __shared__ __attribute__((aligned(1024))) f16 lds[Tile##size##_##name::LDS];                               \
         gemm_tile<Tile##size##_##name, T>(a, lds);                                                                  \
-    }                                                                                                              \
+    }
+#define NS(size, name, T)                                                                                          \
     extern "C" __global__ __launch_bounds__(Tile##size##_##name::THREADS) void thvm_ns_##size##_##name(NsArgs a) {  \
         __shared__ __attribute__((aligned(1024))) f16 lds[Tile##size##_##name::LDS];                               \
         ns_tile<Tile##size##_##name, T>(a, lds);                                                                    \
     }
 #define TILE(...) Tile<__VA_ARGS__>
-GEMM(256, TILE(256, 256, 2, 4, 1, 2, 4), f16, f16)
-GEMM(128, TILE(128, 128, 2, 2, 1, 2, 4), f16, f16)
-GEMM(64, TILE(64, 64, 2, 2, 1, 4, 4), f16, f16)
-GEMM(256, TILE(256, 256, 2, 4, 2, 1, 4), f32, float)
-GEMM(128, TILE(128, 128, 2, 2, 2, 1, 4), f32, float)
-GEMM(64, TILE(64, 64, 2, 2, 2, 2, 4), f32, float)
+GEMM(256x256, TILE(256, 256, 2, 4, 1, 2, 4), f16, f16)
+GEMM(128x128, TILE(128, 128, 2, 2, 1, 4, 4), f16, f16)
+GEMM(64x64, TILE(64, 64, 2, 2, 1, 4, 4), f16, f16)
+GEMM(256x256, TILE(256, 256, 2, 4, 2, 1, 4), f32, float)
+GEMM(128x128, TILE(128, 128, 2, 2, 2, 2, 4), f32, float)
+GEMM(64x64, TILE(64, 64, 2, 2, 2, 2, 4), f32, float)
+NS(256x256, f16, f16)
+NS(128x128, f16, f16)
+NS(64x64, f16, f16)
+NS(256x256, f32, float)
+NS(128x128, f32, float)
+NS(64x64, f32, float)
 
 #define PER_TYPE(PL, name, T)                                                                                      \
-    extern "C" __global__ __launch_bounds__(256) void thvm_gemm_join_##name(GemmArgs a) { gemm_join<PL, T>(a); }    \
-    extern "C" __global__ __launch_bounds__(256) void thvm_few_join_##name(GemmArgs a) { gemm_join<1, T>(a); }      \
-    extern "C" __global__ __launch_bounds__(512) void thvm_pack_sizes_##name(PackArgs a) { pack_sizes<T>(a); }      \
-    extern "C" __global__ __launch_bounds__(256) void thvm_pack_##name(PackArgs a) { pack_tile<PL, T, false>(a, nullptr); } \
+    extern "C" __global__ __launch_bounds__(512) void thvm_pack_sizes_##name(PackSet s) {                           \
+        const u32 i = pack_of(s, blockIdx.x);                                                                       \
+        pack_sizes<T>(s.p[i], blockIdx.x - s.first[i]);                                                             \
+    }                                                                                                              \
+    extern "C" __global__ __launch_bounds__(256) void thvm_pack_##name(PackSet s) {                                 \
+        const u32 i = pack_of(s, blockIdx.x);                                                                       \
+        pack_tile<PL, T, false>(s.p[i], nullptr, blockIdx.x - s.first[i]);                                          \
+    }                                                                                                              \
     extern "C" __global__ __launch_bounds__(256) void thvm_muon_pack_##name(PackArgs a, MuonArgs m) {               \
-        pack_tile<PL, T, true>(a, &m);                                                                              \
+        pack_tile<PL, T, true>(a, &m, blockIdx.x);                                                                              \
     }                                                                                                              \
     extern "C" __global__ __launch_bounds__(256) void thvm_muon_momentum_##name(MuonArgs m) { muon_momentum<T>(m); } \
     extern "C" __global__ __launch_bounds__(1024) void thvm_sum_parts_##name(u64 part, u64 out, u32 C, u32 parts) { \
         sum_parts<T>((const glob<float> *)part, (glob<T> *)out, C, parts);                                                      \
     }                                                                                                              \
-    extern "C" __global__ __launch_bounds__(512) void thvm_few1_##name(GemmArgs a) { few_rows<T, 1>(a); }           \
-    extern "C" __global__ __launch_bounds__(512) void thvm_few4_##name(GemmArgs a) { few_rows<T, 4>(a); }           \
-    extern "C" __global__ __launch_bounds__(512) void thvm_few16_##name(GemmArgs a) { few_rows<T, 16>(a); }
+    extern "C" __global__ __launch_bounds__(512) void thvm_few1_##name(GemmArgs a) { few_rows<T, 1, 16>(a); }       \
+    extern "C" __global__ __launch_bounds__(512) void thvm_few4_##name(GemmArgs a) { few_rows<T, 4, 16>(a); }       \
+    extern "C" __global__ __launch_bounds__(512) void thvm_few16_##name(GemmArgs a) { few_rows<T, 16, 16>(a); }     \
+    extern "C" __global__ __launch_bounds__(512) void thvm_few1n_##name(GemmArgs a) { few_rows<T, 1, 4>(a); }       \
+    extern "C" __global__ __launch_bounds__(512) void thvm_few4n_##name(GemmArgs a) { few_rows<T, 4, 4>(a); }       \
+    extern "C" __global__ __launch_bounds__(512) void thvm_few16n_##name(GemmArgs a) { few_rows<T, 16, 4>(a); }
 PER_TYPE(1, f16, f16)
 PER_TYPE(2, f32, float)
