@@ -211,14 +211,17 @@ int thvm_hip_layer_norm_grad(u32 dx, u32 dgamma, u32 dbeta, u32 dy, u32 x, u32 m
     if (!cols) return THVM_HIP_OK;
     const u64 vecs = div_up(cols, 16 / esize(dtype));
     const int wgrad = dgamma || dbeta, half = dtype == DTYPE_F16;
-    /* the kernels' shapes (norm_kernels.hip) */
+    /* The kernels' shapes (norm_kernels.hip): lanes a row, vectors a lane, and
+     * workgroups, two a compute unit: of 8192x4096 in f16 52 us, against 58 with
+     * one and 61 with three, whose partial sums are longer. */
+    const u32 full = 2 * hipb.n_cu;
     u32 g = 0, nv = 0;
     if (vecs <= (half ? 128 : 256)) for (g = 64, nv = 1; nv * g < vecs;) nv *= 2;
-    else if (vecs <= (half ? 512 : 1024)) for (g = 256, nv = half ? 1 : 2; nv * g < vecs;) nv *= 2;
-    else if (vecs <= (half ? 2048 : 4096)) for (g = 512, nv = half ? 2 : 4; nv * g < vecs;) nv *= 2;
+    else if (vecs <= (half ? 256 : 512)) for (g = 256, nv = half ? 1 : 2; nv * g < vecs;) nv *= 2;
+    else if (vecs <= (half ? 2048 : 4096)) for (g = 512, nv = half ? 1 : 2; nv * g < vecs;) nv *= 2;
     u32 parts;
     if (g) {
-        const u32 per = g < 256 ? 256 / g : 1, full = hipb.n_cu * (g == 512 ? 1 : 2);
+        const u32 per = g < 256 ? 256 / g : 1;
         parts = (u32)(div_up(rows, per) < full ? div_up(rows, per) : full);
     } else parts = (u32)(div_up(rows, 64) < 256 ? div_up(rows, 64) : 256);
     Carve c = {0, 0};
@@ -250,7 +253,7 @@ int thvm_hip_layer_norm_grad(u32 dx, u32 dgamma, u32 dbeta, u32 dy, u32 x, u32 m
     }
     if (wgrad && !rc) {
         snprintf(name, sizeof name, "thvm_lnb_%s_cols", tname(dtype));
-        rc = launch1(name, div_up(2ull * cols, 64), 1, 1, 1024, &a);
+        rc = launch1(name, div_up(2ull * cols, 32), 1, 1, 1024, &a);
     }
     operands_written(o, 9);
     return rc;
@@ -274,7 +277,7 @@ static void packed_carve(Packed *p, Carve *c, u32 dtype) {
 }
 
 /* A product's tile and K splits: C [M][N] over K. */
-typedef struct { u32 T, tm, tn, splits, lanes; f32 time; const char *name; } Plan;
+typedef struct { u32 T, tm, tn, splits, lanes; f32 time; const char *name; u32 tiles; } Plan;
 
 /* Tiles, largest first: the larger, the fewer bytes per product, and the fewer
  * workgroups. What each takes, in us, as measured on products of 512 to 4096
@@ -287,35 +290,39 @@ static const struct {
     f32 unit[2], fixed[2], join;
 } TILES[] = {
     {256, 512, 1, "256x256", {0.41f, 1.15f}, {10, 18}, 15},
+    {192, 256, 1, "192x192", {0.27f, 0.75f}, {8, 12}, 10},     /* of a symmetric product only */
     {128, 256, 1, "128x128", {0.13f, 0.335f}, {6, 9}, 5},
     {64, 256, 2, "64x64", {0.055f, 0.11f}, {5, 6}, 3},
 };
+#define TILE_SYM 1
 
-/* The tile and splits that the estimate puts first. */
-static Plan plan_of(u32 M, u32 N, u32 K, u32 dtype) {
+/* The tile and splits that the estimate puts first, for `count` products of
+ * one shape; sym: C is symmetric, and only its tiles on and above the diagonal
+ * are computed. */
+static Plan plan_of(u32 M, u32 N, u32 K, u32 dtype, u32 count, int sym) {
     const u32 cu = hipb.n_cu ? hipb.n_cu : 256, f = dtype == DTYPE_F32;
     const f32 units = (f32)(round_up(K, 64) / 16);
     Plan best;
     memset(&best, 0, sizeof best);
-    f32 least = 0;
     for (u32 i = 0; i < sizeof TILES / sizeof TILES[0]; i++) {
+        if (i == TILE_SYM && !sym) continue;
         const u32 tm = (u32)div_up(M, TILES[i].T), tn = (u32)div_up(N, TILES[i].T);
-        const u64 tiles = (u64)tm * tn;
+        const u64 tiles = sym ? (u64)tm * (tm + 1) / 2 : (u64)tm * tn;
         for (u32 s = 1; s <= 16; s *= 2) {
-            if (s > 1 && (tiles > COUNTS || units / s < 16)) break;
-            const u64 wgs = tiles * s, rounds = div_up(wgs, (u64)cu * TILES[i].slots);
+            if (s > 1 && (tiles * count > COUNTS || units / s < 16)) break;
+            const u64 wgs = tiles * count * s, rounds = div_up(wgs, (u64)cu * TILES[i].slots);
             /* two workgroups of a compute unit take 1.9 times one's time */
-            const f32 share = TILES[i].slots == 2 && wgs > cu ? (rounds > 1 ? 1.9f * rounds : 1.9f) : (f32)rounds;
-            const f32 t = TILES[i].fixed[f] + share * units / s * TILES[i].unit[f] + (s > 1 ? TILES[i].join + s + (f32)wgs * TILES[i].T * TILES[i].T * 4 / 3e6f : 0);
-            if (best.T && t >= least) continue;
-            least = t;
-            best = (Plan){TILES[i].T, tm, tn, s, TILES[i].lanes, t, TILES[i].name};
+            const f32 share = TILES[i].slots == 2 && wgs > cu ? 1.9f * (f32)rounds : (f32)rounds;
+            const f32 t = TILES[i].fixed[f] + share * units / s * TILES[i].unit[f] +
+                          (s > 1 ? TILES[i].join + s + (f32)wgs * TILES[i].T * TILES[i].T * 4 / 3e6f : 0);
+            if (best.T && t >= best.time) continue;
+            best = (Plan){TILES[i].T, tm, tn, s, TILES[i].lanes, t, TILES[i].name, (u32)tiles};
         }
     }
     return best;
 }
 
-static u64 plan_part_bytes(const Plan *p) { return p->splits > 1 ? 4ull * p->tm * p->tn * p->splits * p->T * p->T : 0; }
+static u64 plan_part_bytes(const Plan *p) { return p->splits > 1 ? 4ull * p->tiles * p->splits * p->T * p->T : 0; }
 
 /* The product of two packed operands with its epilogue (a: out, z, bias, res, act). */
 static int product(const Plan *pl, const Packed *pa, const Packed *pb, u32 M, u32 N, u32 dtype, u64 part, GemmArgs a) {
@@ -325,7 +332,7 @@ static int product(const Plan *pl, const Packed *pa, const Packed *pb, u32 M, u3
     a.tm = pl->tm; a.tn = pl->tn; a.splits = pl->splits;
     a.part = part; a.count = B.counts;
     snprintf(name, sizeof name, "thvm_gemm_%s_%s", pl->name, tname(dtype));
-    return launch1(name, (u64)pl->tm * pl->tn, pl->splits, 1, pl->lanes, &a);
+    return launch1(name, pl->tiles, pl->splits, 1, pl->lanes, &a);
 }
 
 /* A matrix [R][C] to pack (times act'(z) where z is given): `rows` with its
@@ -461,7 +468,7 @@ int thvm_hip_linear(u32 y, u32 z, u32 x, u32 w, u32 bias, u32 res, u32 act, u32 
     memset(&a, 0, sizeof a);
     a.out = addr(y); a.z = addr(z); a.bias = addr(bias); a.res = addr(res); a.act = act;
     int rc;
-    const Plan pl = plan_of(m, n, k, dtype);
+    const Plan pl = plan_of(m, n, k, dtype, 1, 0);
     /* packing takes a launch and the operands' bytes twice over (f32: two launches, three times) */
     const f32 packed = pl.time + (dtype == DTYPE_F16 ? 6 : 12) + (f32)((double)k * (m + (double)n) * 10 / 4e6);
     if (!k || (few_fits(m, k, n, dtype) && (m <= 16 || (m <= 64 && few_time(m, k, n, dtype) < packed)))) {
@@ -504,7 +511,7 @@ int thvm_hip_linear_grad(u32 dx, u32 dw, u32 db, u32 dy, u32 z, u32 x, u32 w, u3
     if (!m) dx = 0;
     if (!n) dw = db = 0;
     if (!dx && !dw && !db) return THVM_HIP_OK;
-    const Plan px_ = plan_of(m, k, n, dtype), pw_ = plan_of(k, n, m, dtype);
+    const Plan px_ = plan_of(m, k, n, dtype, 1, 0), pw_ = plan_of(k, n, m, dtype, 1, 0);
     Packed zr = packed_of(m, n, px_.T), wr = packed_of(k, n, px_.T);       /* dx = dz W^T */
     Packed xc = packed_of(k, m, pw_.T), zc = packed_of(n, m, pw_.T);       /* dW = x^T dz */
     Source src[3] = {{addr(dy), addr(z), act, m, n, dx ? &zr : NULL, dw ? &zc : NULL, addr(db)}};
@@ -547,30 +554,68 @@ int thvm_hip_linear_grad(u32 dx, u32 dw, u32 db, u32 dy, u32 z, u32 x, u32 w, u3
 /* X and A = X X^T are packed times 2^14, B = b A + c A^2 times 2^13: |X| and
  * |A| stay under 1.5 and |B| under 2.9, so all of them stay under 2^16 */
 
-static int muon_chunk(const u32 *param, const u32 *grad, const u32 *m, u32 count, u32 rows, u32 cols, f32 keep, f32 step,
-                      f32 beta, int nesterov, u32 steps, u32 dtype, u32 tile) {
+/* What a step on matrices of one shape works with: the padded sides of X [n][w],
+ * the plans of X X^T, A A and B X, and bytes of X, of A and of a matrix's all. */
+typedef struct {
+    u32 tall, n, w, np, wp;
+    Plan gram, square, apply;
+    u64 xb, ab, stride, part;
+} MuonPlan;
+
+static MuonPlan muon_plan(u32 rows, u32 cols, u32 dtype, u32 count) {
+    MuonPlan p;
+    memset(&p, 0, sizeof p);
+    p.tall = rows > cols;
+    p.n = p.tall ? cols : rows;
+    p.w = p.tall ? rows : cols;
+    p.gram = plan_of(p.n, p.n, p.w, dtype, count, 1);
+    p.square = plan_of(p.n, p.n, p.n, dtype, count, 1);
+    p.apply = plan_of(p.n, p.w, p.n, dtype, count, 0);
+    /* every product finds whole tiles; what no tile writes stays the packing's zeros */
+    const u32 t[3] = {p.gram.T, p.square.T, p.apply.T};
+    for (int i = 0; i < 3; i++) {
+        const u32 np = (u32)round_up(p.n, t[i]);
+        if (np > p.np) p.np = np;
+    }
+    p.wp = (u32)round_up(p.w, p.apply.T);
+    const u64 planes = dtype == DTYPE_F16 ? 1 : 2;
+    p.xb = round_up(2 * planes * p.np * p.wp, 1024);
+    p.ab = round_up(2 * planes * p.np * p.np, 1024);
+    p.stride = 3 * p.xb + 2 * p.ab;      /* X, X^T twice, A, B */
+    const u64 parts[3] = {plan_part_bytes(&p.gram), plan_part_bytes(&p.square), plan_part_bytes(&p.apply)};
+    for (int i = 0; i < 3; i++)
+        if (parts[i] > p.part) p.part = parts[i];
+    return p;
+}
+
+static int ns_product(const Plan *pl, NsArgs *g, u32 count, u32 dtype) {
     char name[48];
-    const int tall = rows > cols;
-    const u32 n = tall ? cols : rows, w = tall ? rows : cols;
-    const u32 np = (u32)round_up(n, tile), wp = (u32)round_up(w, tile);
-    const u64 pl = dtype == DTYPE_F16 ? 1 : 2, xb = round_up(2ull * pl * np * wp, 1024), ab = round_up(2ull * pl * np * np, 1024);
+    g->tm = pl->tm; g->tn = pl->tn; g->splits = pl->splits;
+    snprintf(name, sizeof name, "thvm_ns_%s_%s", pl->name, tname(dtype));
+    return launch1(name, pl->tiles, pl->splits, count, pl->lanes, g);
+}
+
+static int muon_chunk(const MuonPlan *q, const u32 *param, const u32 *grad, const u32 *m, u32 count, u32 rows, u32 cols, f32 keep,
+                      f32 step, f32 beta, int nesterov, u32 steps, u32 dtype) {
+    char name[48];
+    const u32 tall = q->tall, n = q->n, w = q->w, np = q->np, wp = q->wp;
+    const u64 xb = q->xb, ab = q->ab, stride = q->stride;
     MuonArgs mu;
     memset(&mu, 0, sizeof mu);
     mu.numel = (u64)rows * cols;
     mu.blocks = (u32)(div_up(mu.numel, 1024) < 1024 ? div_up(mu.numel, 1024) : 1024);
     mu.nesterov = nesterov != 0;
     mu.beta = beta;
-    /* a matrix's operands, `stride` bytes in all: X, X^T twice, A, B */
-    const u64 stride = 3 * xb + 2 * ab;
+    NsArgs a;
+    memset(&a, 0, sizeof a);
     u64 ops = 0;
     Carve c = {0, 0};
     for (int pass = 0; pass < 2; pass++) {
         ops = carve(&c, stride * count + PACK_SLACK);
         mu.sums = carve(&c, 8ull * mu.blocks * count);
+        a.part = carve(&c, q->part * count);
         if (!pass && !carve_reserve(&c)) return THVM_HIP_ENOMEM;
     }
-    NsArgs a;
-    memset(&a, 0, sizeof a);
     for (u32 i = 0; i < count; i++) {
         a.param[i] = addr(param[i]);
         mu.grad[i] = addr(grad[i]);
@@ -581,7 +626,7 @@ static int muon_chunk(const u32 *param, const u32 *grad, const u32 *m, u32 count
     if (rc) return rc;
     PackArgs p;
     memset(&p, 0, sizeof p);
-    const u64 X = ops, A = ops + 3 * xb, B = A + ab;
+    const u64 X = ops, A = ops + 3 * xb, Bm = A + ab;
     u64 xt = ops + xb, xt2 = ops + 2 * xb;
     p.R = rows; p.C = cols; p.stride = stride;
     p.pn = tall ? xt : X; p.Rn = tall ? wp : np; p.KBn = (tall ? np : wp) / 16;
@@ -590,25 +635,23 @@ static int muon_chunk(const u32 *param, const u32 *grad, const u32 *m, u32 count
     void *pp[] = {&p, &mu};
     snprintf(name, sizeof name, "thvm_muon_pack_%s", tname(dtype));
     rc = launch(name, (u64)(p.Rn / 64) * p.ctiles, count, 1, 256, pp);
-    snprintf(name, sizeof name, "thvm_ns_%ux%u_%s", tile, tile, tname(dtype));
-    const u32 tn = np / tile, tw = wp / tile, lanes = tile == 256 ? 512 : 256, half = tn * (tn + 1) / 2;
-    a.stride = stride; a.n = n; a.w = w; a.tall = (u32)tall; a.keep = keep; a.step = step;
+    a.stride = stride; a.n = n; a.w = w; a.tall = tall; a.keep = keep; a.step = step; a.count = B.counts;
     for (u32 s = 0; s < steps && !rc; s++) {
         NsArgs g = a;      /* A = X X^T */
         g.A = g.B = X; g.out = g.out_t = A;
         g.KB = wp / 16; g.KU = (u32)(round_up(w, 64) / 16); g.KBO = g.KBT = np / 16;
-        g.tm = g.tn = tn; g.sym = 1; g.beta = 1.0f / 16384;
-        rc = launch1(name, half, 1, count, lanes, &g);
-        g.A = g.B = g.old = A; g.out = g.out_t = B;      /* B = b A + c A A */
+        g.sym = 1; g.beta = 1.0f / 16384;
+        rc = ns_product(&q->gram, &g, count, dtype);
+        g.A = g.B = g.old = A; g.out = g.out_t = Bm;      /* B = b A + c A A */
         g.KB = np / 16; g.KU = (u32)(round_up(n, 64) / 16);
         g.alpha = (f32)(NS_B / 2); g.beta = (f32)(NS_C / 32768);
-        if (!rc) rc = launch1(name, half, 1, count, lanes, &g);
-        g.A = B; g.B = xt; g.old = X;                    /* X = a X + B X */
-        g.KBO = wp / 16; g.sym = 0; g.tn = tw;
+        if (!rc) rc = ns_product(&q->square, &g, count, dtype);
+        g.A = Bm; g.B = xt; g.old = X;                    /* X = a X + B X */
+        g.KBO = wp / 16; g.sym = 0;
         g.last = s + 1 == steps;
         g.out = g.last ? 0 : X; g.out_t = g.last ? 0 : xt2;
         g.alpha = (f32)(g.last ? NS_A / 16384 : NS_A); g.beta = g.last ? 1.0f / (1 << 27) : 1.0f / 8192;
-        if (!rc) rc = launch1(name, (u64)tn * tw, 1, count, lanes, &g);
+        if (!rc) rc = ns_product(&q->apply, &g, count, dtype);
         const u64 t = xt; xt = xt2; xt2 = t;
     }
     return rc;
@@ -632,21 +675,17 @@ int thvm_hip_muon_step(const u32 *param, const u32 *grad, const u32 *m, u32 coun
                 return refuse(op, "an output is also another operand");
     }
     if (!numel || !count) return THVM_HIP_OK;
-    const u32 cu = hipb.n_cu ? hipb.n_cu : 256;
-    u32 tile = 256;
-    while (tile > 64 && count * div_up(rows, tile) * div_up(cols, tile) < cu * 3 / 4) tile /= 2;
-    const u64 n = round_up(rows < cols ? rows : cols, tile), w = round_up(rows < cols ? cols : rows, tile);
-    const u64 each = (dtype == DTYPE_F16 ? 2ull : 4ull) * (3 * n * w + 2 * n * n);
     /* as many matrices at once as a launch names, in 4 GiB of workspace */
-    u64 at_once = (4ull << 30) / each;
-    if (at_once < 1) at_once = 1;
-    if (at_once > MUON_MAX) at_once = MUON_MAX;
+    u64 at_once = count < MUON_MAX ? count : MUON_MAX;
+    MuonPlan q = muon_plan(rows, cols, dtype, (u32)at_once);
+    while (at_once > 1 && at_once * (q.stride + q.part) > (4ull << 30)) q = muon_plan(rows, cols, dtype, (u32)--at_once);
     const f32 keep = (f32)(1.0 - (double)lr * weight_decay), step = (f32)((double)lr * scale);
     int rc = THVM_HIP_OK;
     for (u32 i = 0; i < count && !rc; i += (u32)at_once) {
         const u32 nc = count - i < at_once ? count - i : (u32)at_once;
+        if (nc != at_once) q = muon_plan(rows, cols, dtype, nc);
         for (u32 j = i; j < i + nc; j++) hipb_operand(param[j]), hipb_operand(grad[j]), hipb_operand(m[j]);
-        rc = muon_chunk(param + i, grad + i, m + i, nc, rows, cols, keep, step, beta, nesterov != 0, steps, dtype, tile);
+        rc = muon_chunk(&q, param + i, grad + i, m + i, nc, rows, cols, keep, step, beta, nesterov != 0, steps, dtype);
         for (u32 j = i; j < i + nc; j++) pool_mark_device_write(param[j]), pool_mark_device_write(m[j]);
     }
     return rc;

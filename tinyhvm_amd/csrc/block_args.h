@@ -75,11 +75,11 @@ typedef struct {
 /* new = alpha old + beta A B^T over packed operands, see ns_tile */
 typedef struct {
     u64 A, B, old, out, out_t; /* matrix z's operands lie z * stride bytes further */
-    u64 stride;
+    u64 stride, part, count;   /* part, count: as in GemmArgs, matrix by matrix */
     u64 param[MUON_MAX];
     u32 KB, KU;                /* blocks of k: in memory, and multiplied */
     u32 KBO, KBT;              /* of old and out, and of out_t */
-    u32 tm, tn, sym, pad;
+    u32 tm, tn, sym, splits;
     u32 n, w, tall, last;
     f32 alpha, beta, keep, step;
 } NsArgs;

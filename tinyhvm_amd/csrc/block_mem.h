@@ -27,6 +27,17 @@ __device__ __forceinline__ void load_n(const glob<T> *row, u32 e, u32 n, float *
     }
 }
 
+// the same, as they are
+template <typename T, u32 N>
+__device__ __forceinline__ any_vec<T, N> load_raw(const glob<T> *row, u32 e, u32 n) {
+    any_vec<T, N> p;
+    if (e + N <= n) p = *(const glob<any_vec<T, N>> *)(row + e);
+    else
+#pragma unroll
+        for (u32 j = 0; j < N; j++) p[j] = e + j < n ? row[e + j] : (T)0.0f;
+    return p;
+}
+
 template <typename T, u32 N>
 __device__ __forceinline__ void store_n(glob<T> *row, u32 e, u32 n, const float *in) {
     if (e + N <= n) {

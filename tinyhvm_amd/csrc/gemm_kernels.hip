@@ -78,7 +78,7 @@ __device__ __forceinline__ float act_slope(u32 act, float z) {
     }
 }
 
-// The same of 8 values: one choice for all of them.
+// The same of N values: one choice for all of them.
 #define ACT_CASES(f, ...)                                                                                          \
     switch (act) {                                                                                                 \
     case ACT_RELU: ACT_EACH(f(ACT_RELU, z[j]), __VA_ARGS__) break;                                                 \
@@ -87,12 +87,12 @@ __device__ __forceinline__ float act_slope(u32 act, float z) {
     case ACT_SILU: ACT_EACH(f(ACT_SILU, z[j]), __VA_ARGS__) break;                                                 \
     default: break;                                                                                                \
     }
-#define ACT_EACH(e, op) _Pragma("unroll") for (u32 j = 0; j < 8; j++) v[j] op e;
-__device__ __forceinline__ void act8(u32 act, float *v) {
+#define ACT_EACH(e, op) _Pragma("unroll") for (u32 j = 0; j < N; j++) v[j] op e;
+template <u32 N> __device__ __forceinline__ void act_n(u32 act, float *v) {
     const float *z = v;
     ACT_CASES(act_of, =)
 }
-__device__ __forceinline__ void slope8(u32 act, const float *z, float *v) { ACT_CASES(act_slope, *=) }
+template <u32 N> __device__ __forceinline__ void slope_n(u32 act, const float *z, float *v) { ACT_CASES(act_slope, *=) }
 
 template <typename T> __device__ __forceinline__ void load8(const glob<T> *row, u32 e, u32 n, float *out) { load_n<T, 8>(row, e, n, out); }
 template <typename T> __device__ __forceinline__ void store8(glob<T> *row, u32 e, u32 n, const float *in) { store_n<T, 8>(row, e, n, in); }
@@ -456,7 +456,7 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs &a, f16 *lds) {
                 for (u32 j = 0; j < 8; j++) v[j] += bias[j];
             const u64 at = (u64)r * a.N;
             if (a.z) store8<T>((glob<T> *)a.z + at, c, a.N, v);
-            act8(a.act, v);
+            act_n<8>(a.act, v);
             if (a.res) {
                 if (whole)
 #pragma unroll
@@ -520,9 +520,11 @@ __device__ __forceinline__ void ns_tile(const NsArgs &a, f16 *lds) {
     if (a.sym) tile_upper(blockIdx.x, ti, tj);
     else tile_of(blockIdx.x, a.tm, a.tn, ti, tj);
     f16v acc[TL::MI][TL::NI];
+    const u32 S = a.KU / TL::US, per = (S / TL::TURN + a.splits - 1) / a.splits * TL::TURN, s0 = blockIdx.y * per;
     mainloop<TL>(lds, (const glob<f16> *)(a.A + z * a.stride), (const glob<f16> *)(a.B + z * a.stride), a.KB, a.KB, ti * TL::RBA, tj * TL::RBB,
-                 0, a.KU / TL::US, acc);
+                 s0, s0 + per < S ? s0 + per : S, acc);
     wait_stage<0, 0>();
+    if (a.splits > 1 && !join_splits<TL>(a.part, a.count, blockIdx.z * gridDim.x + blockIdx.x, blockIdx.y, a.splits, acc)) return;
     float *st = (float *)lds + wave * 32 * TL::PITCH;
     const glob<f16> *old = (const glob<f16> *)(a.old + z * a.stride);
     glob<f16> *out = (glob<f16> *)(a.out + z * a.stride), *out_t = (glob<f16> *)(a.out_t + z * a.stride);
@@ -667,61 +669,78 @@ __device__ __forceinline__ u32 pack_of(const PackSet &s, u32 block) {
     return (s.n > 1 && block >= s.first[1]) + (s.n > 2 && block >= s.first[2]);
 }
 
-// What is packed at (r, c .. c + 7): the matrix itself, or dy * act'(z).
-template <typename T>
-__device__ __forceinline__ void source8(const PackArgs &a, u32 r, u32 c, float *v) {
-    load8<T>((const glob<T> *)a.src + (u64)r * a.C, c, a.C, v);
+// What is packed at (r, c .. c + N - 1): the matrix itself, or dy * act'(z).
+template <typename T, u32 N>
+__device__ __forceinline__ void source(const PackArgs &a, u32 r, u32 c, float *v) {
+    load_n<T, N>((const glob<T> *)a.src + (u64)r * a.C, c, a.C, v);
     if (a.z) {
-        float z[8];
-        load8<T>((const glob<T> *)a.z + (u64)r * a.C, c, a.C, z);
-        slope8(a.act, z, v);
+        float z[N];
+        load_n<T, N>((const glob<T> *)a.z + (u64)r * a.C, c, a.C, z);
+        slope_n<N>(a.act, z, v);
     }
 }
 
 // The largest values of a matrix's rows and columns (as size words, a part a
 // column tile of 512 and a row tile of a.rt) and the columns' sums.
-// 8 waves, each every 8th row of the tile, a lane 8 columns; four rows are
-// asked for at a time.
-template <typename T>
-__device__ __forceinline__ void pack_sizes(const PackArgs &a, u32 block) {
-    __shared__ u32 lw[8][512];
-    __shared__ float ls[8][512];
-    const u32 lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, bx = block % a.row_parts, by = block / a.row_parts;
+// 8 waves, each every 8th row of the tile, a lane 8 columns; two rows are
+// asked for at a time. Magnitudes compare as their bits do, and infinities and
+// NaN are the largest of all: a tile that holds one is gone through again,
+// with the words that keep the largest finite value beside the mark.
+template <typename T, bool MARKS>
+__device__ __forceinline__ bool pack_sizes_of(const PackArgs &a, u32 bx, u32 by, u32 (*lw)[512], float (*ls)[512]) {
+    const u32 lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     const u32 c = bx * 512u + lane * 8u;
     const u64 r0 = (u64)by * a.rt, r1 = r0 + a.rt < a.R ? r0 + a.rt : a.R;
     u32 cw[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     float cs[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    for (u64 r = r0 + wave; r < r1; r += 32) {
-        float v[4][8];
+    for (u64 r = r0 + wave; r < r1; r += 16) {
+        float v[2][8];
 #pragma unroll
-        for (u32 q = 0; q < 4; q++)
-            if (r + q * 8 < r1 && c < a.C) source8<T>(a, (u32)r + q * 8, c, v[q]);
+        for (u32 q = 0; q < 2; q++)
+            if (r + q * 8 < r1 && c < a.C) source<T, 8>(a, (u32)r + q * 8, c, v[q]);
             else
 #pragma unroll
                 for (u32 j = 0; j < 8; j++) v[q][j] = 0.0f;
 #pragma unroll
-        for (u32 q = 0; q < 4; q++) {
+        for (u32 q = 0; q < 2; q++) {
             u32 rw = 0;
 #pragma unroll
             for (u32 j = 0; j < 8; j++) {
-                const u32 w = size_word(v[q][j]);
-                rw = size_join(rw, w);
-                cw[j] = size_join(cw[j], w);
+                const u32 w = MARKS ? size_word(v[q][j]) : __float_as_uint(v[q][j]) & 0x7FFFFFFFu;
+                rw = MARKS ? size_join(rw, w) : max(rw, w);
+                cw[j] = MARKS ? size_join(cw[j], w) : max(cw[j], w);
                 cs[j] += v[q][j];
             }
             if (a.row_part && r + q * 8 < r1) {
 #pragma unroll
-                for (int d = 32; d; d >>= 1) rw = size_join(rw, __shfl_xor(rw, d));
+                for (int d = 32; d; d >>= 1) {
+                    const u32 o = __shfl_xor(rw, d);
+                    rw = MARKS ? size_join(rw, o) : max(rw, o);
+                }
                 if (lane == 0) ((glob<u32> *)a.row_part)[(u64)bx * a.R + r + q * 8] = rw;
             }
         }
     }
-    if (!a.col_part && !a.sum_part) return;
+    bool mark = false;
 #pragma unroll
-    for (u32 j = 0; j < 8; j++) lw[wave][lane * 8 + j] = cw[j], ls[wave][lane * 8 + j] = cs[j];
-    __syncthreads();
+    for (u32 j = 0; j < 8; j++) {
+        const u32 at = lane * 8 + j;
+        lw[wave][at] = cw[j], ls[wave][at] = cs[j], mark |= cw[j] >= 0x7F800000u;
+    }
+    return mark;
+}
+
+template <typename T>
+__device__ __forceinline__ void pack_sizes(const PackArgs &a, u32 block) {
+    __shared__ u32 lw[8][512];
+    __shared__ float ls[8][512];
+    const u32 bx = block % a.row_parts, by = block / a.row_parts;
+    if (__syncthreads_or(pack_sizes_of<T, false>(a, bx, by, lw, ls))) {
+        pack_sizes_of<T, true>(a, bx, by, lw, ls);
+        __syncthreads();
+    }
     const u32 t = threadIdx.x, ct = bx * 512u + t;
-    if (ct >= a.C) return;
+    if (ct >= a.C || (!a.col_part && !a.sum_part)) return;
     u32 w = lw[0][t];
     float s = ls[0][t];
 #pragma unroll
@@ -794,7 +813,7 @@ __device__ __forceinline__ void pack_tile(const PackArgs &a, const MuonArgs *mu,
                 }
 #pragma unroll
                 for (u32 k = 0; k < 8; k++) v[k] *= unit_lds;
-            } else source8<T>(a, r, c, v);
+            } else source<T, 8>(a, r, c, v);
         }
         if (a.pt || a.sum_part)
 #pragma unroll
@@ -998,6 +1017,10 @@ GEMM(64x64, TILE(64, 64, 2, 2, 1, 4, 4), f16, f16)
 GEMM(256x256, TILE(256, 256, 2, 4, 2, 1, 4), f32, float)
 GEMM(128x128, TILE(128, 128, 2, 2, 2, 2, 4), f32, float)
 GEMM(64x64, TILE(64, 64, 2, 2, 2, 2, 4), f32, float)
+#undef GEMM
+#define NS_TILE(size, TILE, name, T) typedef TILE Tile##size##_##name; NS(size, name, T)
+NS_TILE(192x192, TILE(192, 192, 2, 2, 1, 2, 4), f16, f16)
+NS_TILE(192x192, TILE(192, 192, 2, 2, 2, 1, 4), f32, float)
 NS(256x256, f16, f16)
 NS(128x128, f16, f16)
 NS(64x64, f16, f16)
@@ -1006,10 +1029,6 @@ NS(128x128, f32, float)
 NS(64x64, f32, float)
 
 #define PER_TYPE(PL, name, T)                                                                                      \
-    extern "C" __global__ __launch_bounds__(512) void thvm_pack_sizes_##name(PackSet s) {                           \
-        const u32 i = pack_of(s, blockIdx.x);                                                                       \
-        pack_sizes<T>(s.p[i], blockIdx.x - s.first[i]);                                                             \
-    }                                                                                                              \
     extern "C" __global__ __launch_bounds__(256) void thvm_pack_##name(PackSet s) {                                 \
         const u32 i = pack_of(s, blockIdx.x);                                                                       \
         pack_tile<PL, T, false>(s.p[i], nullptr, blockIdx.x - s.first[i]);                                          \
@@ -1029,3 +1048,8 @@ NS(64x64, f32, float)
     extern "C" __global__ __launch_bounds__(512) void thvm_few16n_##name(GemmArgs a) { few_rows<T, 16, 4>(a); }
 PER_TYPE(1, f16, f16)
 PER_TYPE(2, f32, float)
+// of 32-bit operands: 16-bit ones are packed as they are
+extern "C" __global__ __launch_bounds__(512, 4) void thvm_pack_sizes_f32(PackSet s) {
+    const u32 i = pack_of(s, blockIdx.x);
+    pack_sizes<float>(s.p[i], blockIdx.x - s.first[i]);
+}

@@ -155,8 +155,9 @@ __device__ __forceinline__ void ln_fwd_long(const LnArgs &a) {
 // stay in its registers until the workgroup's rows are done. They are then
 // added over the workgroup's groups and written as one row of the partial
 // sums, which ln_cols adds in row order: no atomics, the same bits each time.
-// The next row's loads are issued before the current row's sums are waited
-// for, where the registers hold two rows.
+// The next row is asked for, as it lies in memory, before the current row's
+// sums are waited for (where the registers hold it), and so is what is added
+// to the current row.
 template <typename T, u32 G, u32 NV>
 __device__ __forceinline__ void ln_bwd(const LnGradArgs &a) {
     constexpr u32 N = Vec<T>::N, PER = G < 256 ? 256 / G : 1;
@@ -173,33 +174,31 @@ __device__ __forceinline__ void ln_bwd(const LnGradArgs &a) {
         for (u32 j = 0; j < N; j++) dg[i][j] = db[i][j] = 0.0f, gm[i][j] = 1.0f;
         if (a.gamma) load_vec<T>((const glob<T> *)a.gamma, (lane + i * G) * N, a.cols, gm[i]);
     }
-    float y1[NV][N], x1[NV][N];
-    u64 r = (u64)blockIdx.x * PER + group;
-    if (AHEAD && r < a.rows)
+    any_vec<T, N> yr[NV], xr[NV], ar[NV];
+    float mean1 = 0.0f, rstd1 = 0.0f;
+    auto ask = [&](u64 r) {
+        mean1 = ((const glob<float> *)a.mean)[r];
+        rstd1 = ((const glob<float> *)a.rstd)[r];
 #pragma unroll
         for (u32 i = 0; i < NV; i++) {
-            load_vec<T>((const glob<T> *)a.dy + r * a.cols, (lane + i * G) * N, a.cols, y1[i]);
-            load_vec<T>((const glob<T> *)a.x + r * a.cols, (lane + i * G) * N, a.cols, x1[i]);
+            yr[i] = load_raw<T, N>((const glob<T> *)a.dy + r * a.cols, (lane + i * G) * N, a.cols);
+            xr[i] = load_raw<T, N>((const glob<T> *)a.x + r * a.cols, (lane + i * G) * N, a.cols);
         }
+    };
+    u64 r = (u64)blockIdx.x * PER + group;
+    if (AHEAD && r < a.rows) ask(r);
     for (u32 slot = 0; r < a.rows; r += step, slot ^= 1u) {
         float y[NV][N], xh[NV][N];
-        const float mean = ((const glob<float> *)a.mean)[r], rstd = ((const glob<float> *)a.rstd)[r];
-        if (!AHEAD)
+        if (!AHEAD) ask(r);
+        const float mean = mean1, rstd = rstd1;
+        if (a.add && a.dx)
 #pragma unroll
-            for (u32 i = 0; i < NV; i++) {
-                load_vec<T>((const glob<T> *)a.dy + r * a.cols, (lane + i * G) * N, a.cols, y1[i]);
-                load_vec<T>((const glob<T> *)a.x + r * a.cols, (lane + i * G) * N, a.cols, x1[i]);
-            }
+            for (u32 i = 0; i < NV; i++) ar[i] = load_raw<T, N>((const glob<T> *)a.add + r * a.cols, (lane + i * G) * N, a.cols);
 #pragma unroll
         for (u32 i = 0; i < NV; i++)
 #pragma unroll
-            for (u32 j = 0; j < N; j++) y[i][j] = y1[i][j], xh[i][j] = (x1[i][j] - mean) * rstd;
-        if (AHEAD && r + step < a.rows)
-#pragma unroll
-            for (u32 i = 0; i < NV; i++) {
-                load_vec<T>((const glob<T> *)a.dy + (r + step) * a.cols, (lane + i * G) * N, a.cols, y1[i]);
-                load_vec<T>((const glob<T> *)a.x + (r + step) * a.cols, (lane + i * G) * N, a.cols, x1[i]);
-            }
+            for (u32 j = 0; j < N; j++) y[i][j] = (float)yr[i][j], xh[i][j] = ((float)xr[i][j] - mean) * rstd;
+        if (AHEAD && r + step < a.rows) ask(r + step);
         // past the row's end dy is 0: nothing there reaches a sum
         float s[2] = {0.0f, 0.0f};
 #pragma unroll
@@ -220,12 +219,11 @@ __device__ __forceinline__ void ln_bwd(const LnGradArgs &a) {
         for (u32 i = 0; i < NV; i++) {
             const u32 e = (lane + i * G) * N;
             if (e >= a.cols) continue;
-            float o[N], ad[N];
-            if (a.add) load_vec<T>((const glob<T> *)a.add + r * a.cols, e, a.cols, ad);
+            float o[N];
 #pragma unroll
             for (u32 j = 0; j < N; j++) {
                 o[j] = rstd * (y[i][j] - c0 - xh[i][j] * c1);
-                if (a.add) o[j] += ad[j];
+                if (a.add) o[j] += (float)ar[i][j];
             }
             store_vec<T>((glob<T> *)a.dx + r * a.cols, e, a.cols, o);
         }
@@ -317,21 +315,22 @@ __device__ __forceinline__ void ln_part_long(const LnGradArgs &a) {
 }
 
 // dgamma and dbeta from `parts` rows of partial sums [2][cols]: a workgroup
-// takes 64 of the 2 * cols columns, its 16 waves every 16th part, and adds
-// the waves' sums in order.
+// takes 32 of the 2 * cols columns, 32 groups of its lanes every 32nd part,
+// and adds the groups' sums in order.
 template <typename T>
 __device__ __forceinline__ void ln_cols(const LnGradArgs &a) {
-    __shared__ float lds[16][64];
-    const u32 lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    const u64 c = (u64)blockIdx.x * 64u + lane, n2 = 2ull * a.cols;
+    __shared__ float lds[32][33];
+    const u32 lane = threadIdx.x & 31u, group = threadIdx.x >> 5;
+    const u64 c = (u64)blockIdx.x * 32u + lane, n2 = 2ull * a.cols;
     float s = 0.0f;
     if (c < n2)
-        for (u32 p = wave; p < a.parts; p += 16) s += ((const glob<float> *)a.part)[p * n2 + c];
-    lds[wave][lane] = s;
+#pragma unroll 8
+        for (u32 p = group; p < a.parts; p += 32) s += ((const glob<float> *)a.part)[p * n2 + c];
+    lds[group][lane] = s;
     __syncthreads();
-    if (wave || c >= n2) return;
+    if (group || c >= n2) return;
 #pragma unroll
-    for (u32 w = 1; w < 16; w++) s += lds[w][lane];
+    for (u32 w = 1; w < 32; w++) s += lds[w][lane];
     glob<T> *out = c < a.cols ? (glob<T> *)a.dgamma : (glob<T> *)a.dbeta;
     if (out) out[c < a.cols ? c : c - a.cols] = (T)s;
 }
@@ -355,6 +354,6 @@ __device__ __forceinline__ void ln_cols(const LnGradArgs &a) {
 LN_ALL(f32)
 LN_ALL(f16)
 LNB_KERNELS(f32, 64, 1) LNB_KERNELS(f32, 64, 2) LNB_KERNELS(f32, 64, 4)
-LNB_KERNELS(f32, 256, 2) LNB_KERNELS(f32, 256, 4) LNB_KERNELS(f32, 512, 4) LNB_KERNELS(f32, 512, 8)
+LNB_KERNELS(f32, 256, 2) LNB_KERNELS(f32, 256, 4) LNB_KERNELS(f32, 512, 2) LNB_KERNELS(f32, 512, 4) LNB_KERNELS(f32, 512, 8)
 LNB_KERNELS(f16, 64, 1) LNB_KERNELS(f16, 64, 2)
-LNB_KERNELS(f16, 256, 1) LNB_KERNELS(f16, 256, 2) LNB_KERNELS(f16, 512, 2) LNB_KERNELS(f16, 512, 4)
+LNB_KERNELS(f16, 256, 1) LNB_KERNELS(f16, 256, 2) LNB_KERNELS(f16, 512, 1) LNB_KERNELS(f16, 512, 2) LNB_KERNELS(f16, 512, 4)
