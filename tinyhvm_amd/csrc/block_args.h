@@ -35,7 +35,8 @@ typedef struct {
     u64 out, z, bias, res;     /* row-major [M][N]; bias [N] */
     u64 part, count;           /* the K splits' sums, and how many of a tile's are there (0 between launches) */
     u32 M, N, KB, tm, tn, splits, act;
-    u32 K, kper, pad;          /* few rows: A is x [M][K], B is W [K][N], kper k a split */
+    u32 K, lda, ldb;           /* operands as they lie */
+    u32 kper;                  /* few rows: A is x [M][K], B is W [K][N], kper k a split */
 } GemmArgs;
 
 /* few rows: the longest K split of a workgroup, whose part of x it holds in LDS */

@@ -27,6 +27,9 @@
 #include "block_mem.h"
 
 typedef f16 h8 __attribute__((ext_vector_type(8)));
+typedef f16 h4 __attribute__((ext_vector_type(4)));
+typedef int i4v __attribute__((ext_vector_type(4)));
+typedef short s4v __attribute__((ext_vector_type(4)));
 typedef float f16v __attribute__((ext_vector_type(16)));   // a 32x32 block's sums
 typedef float f4 __attribute__((ext_vector_type(4)));
 
@@ -132,7 +135,6 @@ __device__ __forceinline__ float exact_dot(const glob<f16> *A, const glob<f16> *
 
 // ---- the product ----
 
-typedef __attribute__((address_space(1))) const void *gptr;
 typedef __attribute__((address_space(3))) void *lptr;
 
 // Every load to LDS but the last `loads` of this wave and every read of LDS
@@ -164,17 +166,42 @@ struct Tile {
     static_assert((NS - 1) * CK * 1024 <= PACK_SLACK, "loads past the end");
 };
 
-template <bool v> struct Flag { static constexpr bool value = v; };
+template <u32 v> struct Const { static constexpr u32 value = v; };
 
-// The sums of a tile over stages s0 .. s1 - 1. A unit's fragments are read
+// How an operand lies in memory: packed; or, in 16 bits, row-major with k
+// along its rows (ROWS: element (r, k) at r ld + k) or across them (COLS: at
+// k ld + r), rows of a multiple of 8 elements. Those that are not packed go to
+// LDS in chunks of the same 1 KB:
+//   ROWS  two chunks hold 32 rows by 32 k, 64 bytes a row, the row's four 16
+//         bytes turned by the row (octet o at place o ^ (row / 4) % 4), so that
+//         the 16 rows that are read together lie in different banks;
+//   COLS  a chunk holds 16 k by 32 rows, 64 bytes a k, and is turned on the
+//         way to registers (ds_read_b64_tr_b16: of 16 lanes that read 4 k by 16
+//         rows, lane i gets the 4 k of row i).
+// Past the end of K, and past the last row, they read as 0 or as another row,
+// whose sums no one takes.
+enum { PACKED = 0, ROWS, COLS };
+
+// What a wave brings to LDS: where its chunks of a stage are (bytes from a
+// base that moves by `step` a stage), and the k, in the stage, that each of its
+// lanes begins at. Reads past `end` give 0.
+struct Operand {
+    u64 base;         // of the first stage, the tile's first row
+    u64 end;          // of the memory
+    u32 ld, rows;     // ROWS, COLS; rows from the tile's first on
+    u32 K;            // k from the first stage on
+};
+
+// The sums of a tile over n stages. A unit's fragments are read
 // from LDS while the unit before is multiplied; where that begins a stage,
 // the wait for the stage and the barrier come ahead of the reads, so that
 // they too pass behind multiplications. A stage is brought NS - 1 ahead, into
 // the buffer whose last reader has passed that barrier.
-template <typename TL>
-__device__ __forceinline__ void mainloop(f16 *lds, const glob<f16> *A, const glob<f16> *B, u32 KBA, u32 KBB, u32 rb0, u32 cb0, u32 s0, u32 s1,
+template <typename TL, u32 MA, u32 MB>
+__device__ __forceinline__ void mainloop(f16 *lds, const Operand &A, const Operand &B, u64 stride_a, u64 stride_b, u32 n,
                                          f16v (&acc)[TL::MI][TL::NI]) {
-    constexpr u32 PL = TL::PL, NS = TL::NS, Q = TL::Q;
+    constexpr u32 PL = TL::PL, NS = TL::NS, Q = TL::Q, CK = TL::CK;
+    static_assert(PL == 1 || (MA == PACKED && MB == PACKED), "planes are packed");
     const u32 lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const u32 wm = wave / TL::WN, wn = wave % TL::WN;
 #pragma unroll
@@ -183,35 +210,76 @@ __device__ __forceinline__ void mainloop(f16 *lds, const glob<f16> *A, const glo
         for (u32 j = 0; j < TL::NI; j++)
 #pragma unroll
             for (u32 v = 0; v < 16; v++) acc[i][j][v] = 0.0f;
-    if (s0 >= s1) return;
-    const glob<f16> *src[Q];
+    if (!n) return;
+    // a wave's row blocks are all of A or all of B
+    static_assert(TL::RBA % Q == 0, "");
+    const bool of_a = wave * Q < TL::RBA;
+    const u32 mode = of_a ? MA : MB, ld = of_a ? A.ld : B.ld, rows = of_a ? A.rows : B.rows;
+    const u32 rb0 = of_a ? wave * Q : wave * Q - TL::RBA;
+    const u64 stride = of_a ? stride_a : stride_b;        // PACKED: bytes of a row block
+    const u64 end = of_a ? A.end : B.end;
+    const u64 step = mode == PACKED ? CK * 1024u : mode == ROWS ? CK * 32u : (u64)CK * 32u * ld;
+    // this wave's first row (or the last there is), and offsets from there
+    const u32 row0 = mode == PACKED || rb0 * 32 < rows ? rb0 * 32 : rows - 1;
+    u64 base = (of_a ? A.base : B.base) + (mode == PACKED ? rb0 * stride : mode == ROWS ? (u64)row0 * ld * 2u : 0u);
+    u32 off[Q][CK], first[CK], left = of_a ? A.K : B.K;
 #pragma unroll
-    for (u32 q = 0; q < Q; q++) {
-        const u32 b = wave * Q + q;
-        const glob<f16> *base = b < TL::RBA ? A + block_at<PL>(rb0 + b, 0, KBA, 0) : B + block_at<PL>(cb0 + b - TL::RBA, 0, KBB, 0);
-        src[q] = base + (u64)s0 * (TL::CK * 512u) + lane * 8u;
-    }
-    // Past the last stage what follows in memory is brought, for no one to
-    // read, so that the count of loads in flight stays the same (a packed
-    // operand ends PACK_SLACK short of its allocation).
-    auto bring = [&](u32 buf, u32 n) {       // the n-th chunk
-        const u32 q = n / TL::CK, dst = (u32)(uintptr_t)(lptr)lds + (buf * TL::STAGE + (wave * Q + q) * (TL::CK * 512u)) * 2u;
-        switch (n % TL::CK) {                // the offset is part of the instruction
-        case 0: __builtin_amdgcn_global_load_lds((gptr)src[q], (lptr)(uintptr_t)dst, 16, 0, 0); break;
-        case 1: __builtin_amdgcn_global_load_lds((gptr)src[q], (lptr)(uintptr_t)dst, 16, 1024, 0); break;
-        case 2: __builtin_amdgcn_global_load_lds((gptr)src[q], (lptr)(uintptr_t)dst, 16, 2048, 0); break;
-        default: __builtin_amdgcn_global_load_lds((gptr)src[q], (lptr)(uintptr_t)dst, 16, 3072, 0); break;
+    for (u32 c = 0; c < CK; c++) {
+        first[c] = mode == PACKED ? 0 : mode == ROWS ? (c >> 1) * 32 + ((lane & 3u) ^ (lane >> 4)) * 8 : c * 16 + (lane >> 2);
+#pragma unroll
+        for (u32 q = 0; q < Q; q++) {
+            if (mode == PACKED) off[q][c] = (u32)(q * stride) + c * 1024u + lane * 16u;
+            else if (mode == ROWS) {
+                const u32 r = (rb0 + q) * 32 + (c & 1u) * 16 + (lane >> 2);
+                off[q][c] = (((r < rows ? r : rows - 1) - row0) * ld + first[c]) * 2u;
+            } else {
+                const u32 r = (rb0 + q) * 32 + (lane & 3u) * 8;
+                off[q][c] = (first[c] * ld + (r < rows ? r : rows - 8)) * 2u;
+            }
         }
-        if (n % TL::CK == TL::CK - 1) src[q] += TL::CK * 512u;
+    }
+    // Past the last stage too, for no one to read, so that the count of loads
+    // in flight stays the same.
+    auto bring = [&](u32 buf, u32 m) {       // the m-th chunk
+        const u32 q = m / CK, c = m % CK;
+        const u32 dst = (u32)(uintptr_t)(lptr)lds + (buf * TL::STAGE + ((wave * Q + q) * CK + c) * 512u) * 2u;
+        const u32 room = end <= base ? 0u : end - base > 0xFFFFFFE0u ? 0xFFFFFFE0u : (u32)(end - base);
+        const u32 at = first[c] < left ? off[q][c] : 0xFFFFFFF0u;      // past any room
+        // Written out, so that the compiler does not know of it: it would wait
+        // for every load to LDS ahead of each turning read. It has no result
+        // in a register, and wait_stage and the barriers order it.
+        const i4v where = {(int)(u32)base, (int)(u32)(base >> 32), (int)room, 0x00020000};
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"     // m0 is written on purpose
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(dst), "v"(at), "s"(where) : "memory", "m0");
+#pragma clang diagnostic pop
+        if (m == TL::CH - 1) {
+            base += step;
+            left = left > CK / PL * 16u ? left - CK / PL * 16u : 0u;
+        }
     };
     h8 a[2][TL::MI][PL], b[2][TL::NI][PL];
     // the n-th fragment of unit k of a stage
     constexpr u32 FRAGS = (TL::MI + TL::NI) * PL;
+    const u32 turned = (lane & 31u) * 32u + ((lane >> 5) ^ ((lane >> 2) & 3u)) * 8u;                             // ROWS, in elements
+    const u32 across = ((lane >> 5) * 8 + ((lane & 15u) >> 2)) * 32u + ((lane >> 4) & 1u) * 16 + (lane & 3u) * 4;  // COLS
+    auto fragment = [&](auto how, const f16 *block, u32 chunk) -> h8 {
+        constexpr u32 mode = decltype(how)::value;
+        if constexpr (mode == PACKED) return *(const h8 *)(block + chunk * 512u + lane * 8u);
+        else if constexpr (mode == ROWS) return *(const h8 *)(block + (chunk >> 1) * 1024u + (chunk & 1u ? turned ^ 16u : turned));
+        else {
+            typedef __attribute__((address_space(3))) s4v *p;
+            const u32 at = (u32)(uintptr_t)(lptr)block + (chunk * 512u + across) * 2u;
+            const h4 lo = __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((p)(uintptr_t)at));
+            const h4 hi = __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((p)(uintptr_t)(at + 256u)));
+            return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    };
     auto fetch = [&](u32 buf, u32 k, u32 n, h8 (&fa)[TL::MI][PL], h8 (&fb)[TL::NI][PL]) {
-        const f16 *st = lds + buf * TL::STAGE + lane * 8u;
+        const f16 *st = lds + buf * TL::STAGE;
         const u32 p = n / (TL::MI + TL::NI), x = n % (TL::MI + TL::NI);
-        if (x < TL::NI) fb[x][p] = *(const h8 *)(st + ((TL::RBA + wn * TL::NI + x) * TL::CK + k * PL + p) * 512u);
-        else fa[x - TL::NI][p] = *(const h8 *)(st + ((wm * TL::MI + x - TL::NI) * TL::CK + k * PL + p) * 512u);
+        if (x < TL::NI) fb[x][p] = fragment(Const<MB>{}, st + (TL::RBA + wn * TL::NI + x) * (CK * 512u), k * PL + p);
+        else fa[x - TL::NI][p] = fragment(Const<MA>{}, st + (wm * TL::MI + x - TL::NI) * (CK * 512u), k * PL + p);
     };
     // The products of a unit (hi hi, then hi lo and lo hi), between them the
     // reads of the next unit's fragments and, where a stage has begun, the
@@ -230,14 +298,14 @@ __device__ __forceinline__ void mainloop(f16 *lds, const glob<f16> *A, const glo
             acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[i][t >> 1], fb[j][t & 1], acc[i][j], 0, 0, 0);
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
 #pragma unroll
-            for (u32 n = m * RP; n < (m + 1) * RP && n < FRAGS; n++) {
-                fetch(buf, u, n, na, nb);
-                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            for (u32 f = m * RP; f < (m + 1) * RP && f < FRAGS; f++) {
+                fetch(buf, u, f, na, nb);
+                if ((f % (TL::MI + TL::NI) < TL::NI ? MB : MA) == COLS) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+                else __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             }
 #pragma unroll
-            for (u32 n = m * LOADS / MFMAS; n < (m + 1) * LOADS / MFMAS; n++) {
-                bring(into, n);
-                __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+            for (u32 f = m * LOADS / MFMAS; f < (m + 1) * LOADS / MFMAS; f++) {
+                bring(into, f);
             }
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -245,19 +313,19 @@ __device__ __forceinline__ void mainloop(f16 *lds, const glob<f16> *A, const glo
 #pragma unroll
     for (u32 i = 0; i + 1 < NS; i++)
 #pragma unroll
-        for (u32 n = 0; n < TL::CH; n++) bring(i, n);
+        for (u32 f = 0; f < TL::CH; f++) bring(i, f);
     wait_stage<(NS - 2) * TL::CH, 0>();
 #pragma unroll
-    for (u32 n = 0; n < FRAGS; n++) fetch(0, 0, n, a[0], b[0]);
-    for (u32 s = s0, buf = 0; s < s1; s += TL::TURN) {
+    for (u32 f = 0; f < FRAGS; f++) fetch(0, 0, f, a[0], b[0]);
+    for (u32 s = 0, buf = 0; s < n; s += TL::TURN) {
 #pragma unroll
         for (u32 u = 0; u < TL::US * TL::TURN; u++) {
             if ((u + 1) % TL::US == 0) {       // the next unit begins a stage
                 wait_stage<(NS - 3) * TL::CH, TL::READS>();
                 const u32 into = (buf + NS - 1) & (NS - 1);
                 buf = (buf + 1) & (NS - 1);
-                unit(Flag<true>{}, buf, into, 0, a[u & 1], b[u & 1], a[(u + 1) & 1], b[(u + 1) & 1]);
-            } else unit(Flag<false>{}, buf, 0, u + 1, a[u & 1], b[u & 1], a[(u + 1) & 1], b[(u + 1) & 1]);
+                unit(Const<1>{}, buf, into, 0, a[u & 1], b[u & 1], a[(u + 1) & 1], b[(u + 1) & 1]);
+            } else unit(Const<0>{}, buf, 0, u + 1, a[u & 1], b[u & 1], a[(u + 1) & 1], b[(u + 1) & 1]);
         }
     }
 }
@@ -322,6 +390,26 @@ __device__ __forceinline__ bool column_exps(const GemmArgs &a, u32 c, int *ec) {
         ec[j] = exp_of(w);
     }
     return odd;
+}
+
+// The operand of a tile that begins at row r0, from stage s0 on.
+template <typename TL, u32 M>
+__device__ __forceinline__ Operand operand(u64 p, u32 ld, u32 rows, u32 r0, u32 KB, u32 K, u32 s0) {
+    Operand o;
+    const u64 k0 = (u64)s0 * (TL::US * 16u);
+    o.ld = ld;
+    if (M == PACKED) {
+        o.base = p + block_at<TL::PL>(r0 >> 5, 0, KB, 0) * 2u + (u64)s0 * (TL::CK * 1024u);
+        o.end = ~0ull;        // past it: PACK_SLACK
+        o.rows = 0;
+        o.K = ~0u;
+    } else {
+        o.base = p + (M == ROWS ? (u64)r0 * ld + k0 : k0 * ld + r0) * 2u;
+        o.end = p + (M == ROWS ? (u64)rows : (u64)K) * ld * 2u;
+        o.rows = rows - r0;
+        o.K = K > k0 ? K - (u32)k0 : 0u;
+    }
+    return o;
 }
 
 // ---- sums that several workgroups have parts of ----
@@ -398,7 +486,7 @@ __device__ __forceinline__ bool join_splits(u64 part, u64 count, u32 tile, u32 s
 }
 
 // A tile of one product, or of one of its K splits (blockIdx.y).
-template <typename TL, typename T>
+template <typename TL, typename T, u32 MA, u32 MB>
 __device__ __forceinline__ void gemm_tile(const GemmArgs &a, f16 *lds) {
     const u32 wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     u32 ti, tj;
@@ -406,7 +494,9 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs &a, f16 *lds) {
     const u32 S = a.KB / TL::US, per = (S / TL::TURN + a.splits - 1) / a.splits * TL::TURN, s0 = blockIdx.y * per;
     const u32 s1 = s0 + per < S ? s0 + per : S;
     f16v acc[TL::MI][TL::NI];
-    mainloop<TL>(lds, (const glob<f16> *)a.A, (const glob<f16> *)a.B, a.KB, a.KB, ti * TL::RBA, tj * TL::RBB, s0, s1, acc);
+    const Operand A = operand<TL, MA>(a.A, a.lda, a.M, ti * TL::TM, a.KB, a.K, s0);
+    const Operand B = operand<TL, MB>(a.B, a.ldb, a.N, tj * TL::TN, a.KB, a.K, s0);
+    mainloop<TL, MA, MB>(lds, A, B, (u64)a.KB * TL::PL * 1024u, (u64)a.KB * TL::PL * 1024u, s0 < s1 ? s1 - s0 : 0, acc);
     wait_stage<0, 0>();
     if (a.splits > 1 && !join_splits<TL>(a.part, a.count, blockIdx.x, blockIdx.y, a.splits, acc)) return;
     // A lane keeps 8 columns and takes every RPP-th row of them. The residual
@@ -521,8 +611,10 @@ __device__ __forceinline__ void ns_tile(const NsArgs &a, f16 *lds) {
     else tile_of(blockIdx.x, a.tm, a.tn, ti, tj);
     f16v acc[TL::MI][TL::NI];
     const u32 S = a.KU / TL::US, per = (S / TL::TURN + a.splits - 1) / a.splits * TL::TURN, s0 = blockIdx.y * per;
-    mainloop<TL>(lds, (const glob<f16> *)(a.A + z * a.stride), (const glob<f16> *)(a.B + z * a.stride), a.KB, a.KB, ti * TL::RBA, tj * TL::RBB,
-                 s0, s0 + per < S ? s0 + per : S, acc);
+    const u32 s1 = s0 + per < S ? s0 + per : S;
+    const Operand A = operand<TL, PACKED>(a.A + z * a.stride, 0, 0, ti * TL::TM, a.KB, 0, s0);
+    const Operand B = operand<TL, PACKED>(a.B + z * a.stride, 0, 0, tj * TL::TN, a.KB, 0, s0);
+    mainloop<TL, PACKED, PACKED>(lds, A, B, (u64)a.KB * PL * 1024u, (u64)a.KB * PL * 1024u, s0 < s1 ? s1 - s0 : 0, acc);
     wait_stage<0, 0>();
     if (a.splits > 1 && !join_splits<TL>(a.part, a.count, blockIdx.z * gridDim.x + blockIdx.x, blockIdx.y, a.splits, acc)) return;
     float *st = (float *)lds + wave * 32 * TL::PITCH;
@@ -999,21 +1091,26 @@ __device__ __forceinline__ void few_rows(const GemmArgs &a) {
 
 // ---- the kernels ----
 
-#define GEMM(size, TILE, name, T)                                                                                  \
+#define GEMM(size, TILE, name, T, ...)                                                                             \
     typedef TILE Tile##size##_##name;                                                                              \
-    extern "C" __global__ __launch_bounds__(Tile##size##_##name::THREADS) void thvm_gemm_##size##_##name(GemmArgs a) { \
+    GEMM_OF(size, name, T, , PACKED, PACKED)                                                                        \
+    __VA_ARGS__
+#define GEMM_OF(size, name, T, how, MA, MB)                                                                         \
+    extern "C" __global__ __launch_bounds__(Tile##size##_##name::THREADS) void thvm_gemm##how##_##size##_##name(GemmArgs a) { \
         __shared__ __attribute__((aligned(1024))) f16 lds[Tile##size##_##name::LDS];                               \
-        gemm_tile<Tile##size##_##name, T>(a, lds);                                                                  \
+        gemm_tile<Tile##size##_##name, T, MA, MB>(a, lds);                                                          \
     }
+// x W with both as they lie
+#define AS_THEY_LIE(size) GEMM_OF(size, f16, f16, _rc, ROWS, COLS)
 #define NS(size, name, T)                                                                                          \
     extern "C" __global__ __launch_bounds__(Tile##size##_##name::THREADS) void thvm_ns_##size##_##name(NsArgs a) {  \
         __shared__ __attribute__((aligned(1024))) f16 lds[Tile##size##_##name::LDS];                               \
         ns_tile<Tile##size##_##name, T>(a, lds);                                                                    \
     }
 #define TILE(...) Tile<__VA_ARGS__>
-GEMM(256x256, TILE(256, 256, 2, 4, 1, 2, 4), f16, f16)
-GEMM(128x128, TILE(128, 128, 2, 2, 1, 4, 4), f16, f16)
-GEMM(64x64, TILE(64, 64, 2, 2, 1, 4, 4), f16, f16)
+GEMM(256x256, TILE(256, 256, 2, 4, 1, 2, 4), f16, f16, AS_THEY_LIE(256x256))
+GEMM(128x128, TILE(128, 128, 2, 2, 1, 4, 4), f16, f16, AS_THEY_LIE(128x128))
+GEMM(64x64, TILE(64, 64, 2, 2, 1, 4, 4), f16, f16, AS_THEY_LIE(64x64))
 GEMM(256x256, TILE(256, 256, 2, 4, 2, 1, 4), f32, float)
 GEMM(128x128, TILE(128, 128, 2, 2, 2, 2, 4), f32, float)
 GEMM(64x64, TILE(64, 64, 2, 2, 2, 2, 4), f32, float)
