@@ -79,6 +79,11 @@ static hipFunction_t kernel(const char *name) {
 
 /* ---- arguments ---- */
 
+/* Two row blocks of a packed operand of this many k are reached by 32-bit
+ * offsets from one address; and rows, or columns, that the launches can count. */
+#define MAX_SUM (1u << 24)
+#define MAX_SIDE (1u << 28)
+
 static int refuse(const char *op, const char *why) {
     fprintf(stderr, "tinyhvm-hip: %s: %s\n", op, why);
     return THVM_HIP_EINVAL;
@@ -162,7 +167,6 @@ static int ln_shape(u32 rows, u32 cols, u32 dtype, u32 *g, u32 *nv) {
     const u64 vecs = div_up(cols, 16 / esize(dtype));
     *g = vecs <= 256 && (rows >= 1024 || vecs <= 64) ? 64 : vecs <= 1024 && rows >= 256 ? 256 : 1024;
     if (*g == 1024 && vecs <= 256) *g = 256;
-    if (*g == 256 && vecs > 2048) *g = 1024;
     for (*nv = 1; *nv * *g < vecs; *nv *= 2) {}
     return *nv <= (*g == 1024 ? 4u : 8u);
 }
@@ -172,6 +176,7 @@ int thvm_hip_layer_norm(u32 y, u32 mean, u32 rstd, u32 x, u32 gamma, u32 beta, u
     const char *op = "layer_norm";
     if (!dtype_ok(dtype)) return refuse(op, "the type is neither f32 nor f16");
     if (!y || !x) return refuse(op, "no input or no output");
+    if (cols > MAX_SUM) return refuse(op, "rows of more than 2^24 values");
     const u64 n = (u64)rows * cols * esize(dtype), v = cols * esize(dtype), st = rows * 4ull;
     const Operand o[] = {{y, n, 1}, {mean, st, 1}, {rstd, st, 1}, {x, n, 0}, {gamma, v, 0}, {beta, v, 0}};
     const u32 same[][2] = {{0, 3}};
@@ -203,6 +208,7 @@ int thvm_hip_layer_norm_grad(u32 dx, u32 dgamma, u32 dbeta, u32 dy, u32 x, u32 m
     if (!dtype_ok(dtype)) return refuse(op, "the type is neither f32 nor f16");
     if (!dy || !x || !mean || !rstd) return refuse(op, "no gradient, input or statistics");
     if (!dx && !dgamma && !dbeta) return refuse(op, "no output");
+    if (cols > MAX_SUM) return refuse(op, "rows of more than 2^24 values");
     const u64 n = (u64)rows * cols * esize(dtype), v = cols * esize(dtype), st = rows * 4ull;
     const Operand o[] = {{dx, n, 1}, {dgamma, v, 1}, {dbeta, v, 1}, {dy, n, 0}, {x, n, 0},
                          {mean, st, 0}, {rstd, st, 0}, {gamma, v, 0}, {add, n, 0}};
@@ -261,9 +267,6 @@ int thvm_hip_layer_norm_grad(u32 dx, u32 dgamma, u32 dbeta, u32 dy, u32 x, u32 m
 
 /* ---- products ---- */
 
-/* a row block of a packed operand is reached by 32-bit offsets */
-#define MAX_SUM (1u << 24)
-
 /* A packed operand of `rows` rows by `k`, padded to whole tiles. */
 typedef struct { u32 Rp, KB; u64 p, e; } Packed;
 
@@ -279,8 +282,9 @@ static Packed packed_of(u32 rows, u32 k, u32 tile) {
  * 21 us; 2048^3 25 us against 30 in all, 512 x 4096 x 512 12 against 20. A
  * gradient packs dz in any case, and W and x with it for next to nothing
  * (2048^3: 12 us against 11), so it multiplies packed operands (56 us against
- * 60 with W and x as they lie). */
-static int lies_well(u32 cols, u32 dtype) { return dtype == DTYPE_F16 && cols % 8 == 0 && cols; }
+ * 60 with W and x as they lie). A tile reaches up to 64 rows from one address
+ * by 32-bit offsets, which a longer row would pass. */
+static int lies_well(u32 cols, u32 dtype) { return dtype == DTYPE_F16 && cols % 8 == 0 && cols && cols <= MAX_SUM; }
 
 static void packed_carve(Packed *p, Carve *c, u32 dtype) {
     p->p = carve(c, packed_bytes(p, dtype) + PACK_SLACK);
@@ -316,7 +320,7 @@ static Plan plan_of(u32 M, u32 N, u32 K, u32 dtype, u32 count, int sym) {
     Plan best;
     memset(&best, 0, sizeof best);
     for (u32 i = 0; i < sizeof TILES / sizeof TILES[0]; i++) {
-        if (i == TILE_SYM && !sym) continue;
+        if (i == TILE_SYM && (!sym || K > MAX_SUM / 2)) continue;      /* it reaches three row blocks at once */
         const u32 tm = (u32)div_up(M, TILES[i].T), tn = (u32)div_up(N, TILES[i].T);
         const u64 tiles = sym ? (u64)tm * (tm + 1) / 2 : (u64)tm * tn;
         for (u32 s = 1; s <= 16; s *= 2) {
@@ -428,30 +432,42 @@ static int pack(const Source *src, u32 n, u32 dtype) {
     return rc;
 }
 
-/* Few rows: W is read as it lies, by blocks of 1, 4 or 16 rows (few_rows in
- * gemm_kernels.hip). Whether the outputs have counters, or need none. */
-#define FEW_NARROW (4u << 20) /* bytes of W */
-static u32 few_block(u32 m) { return m <= 1 ? 1 : m <= 4 ? 4 : 16; }
+/* Few rows: W is read as it lies, by blocks of 1 or 16 rows (few_rows in
+ * gemm_kernels.hip); two rows take the block of 16, which is at most 6 % slower
+ * for 4 than a block of 4 was (256 x 256) and up to 25 % faster (1024 x 2048). */
+static u32 few_block(u32 m) { return m <= 1 ? 1 : 16; }
+
+/* Strips of 64 bytes of a row of W with K whole, or of 256 bytes with K split
+ * over workgroups: joining splits takes 2 to 4 us, but few narrow strips do not
+ * read a large W as fast as the card can. f32, one row: 1024 x 2048 4.95 us
+ * narrow, 5.7 wide; 1024 x 3000 7.6 and 6.9. 64 rows: 1024 x 1024 (256 workgroups)
+ * 5.5 and 7.9; 512 x 4096 (1024 of them) 14 and 5.8. */
+#define FEW_NARROW (8u << 20) /* bytes of W */
+static int few_narrow(u32 m, u32 k, u32 n, u32 dtype) {
+    if (n < 16 / esize(dtype)) return 1;      /* no wide vector */
+    return k <= FEW_CHUNK && (u64)k * n * esize(dtype) <= FEW_NARROW &&
+           div_up(n, 64 / esize(dtype)) * div_up(m, few_block(m)) <= 256;
+}
+/* Whether the kernels take the shape, and the outputs have counters or need none. */
 static int few_fits(u32 m, u32 k, u32 n, u32 dtype) {
+    if (k && n < 4 / esize(dtype)) return 0;      /* a lane takes 4 bytes of a row at least */
     return div_up(n, 256 / esize(dtype)) * div_up(m, few_block(m)) <= COUNTS || k <= FEW_CHUNK;
 }
 
 /* Its time in us, roughly: W's bytes once a block of rows. */
 static f32 few_time(u32 m, u32 k, u32 n, u32 dtype) {
-    return (f32)(8 + (double)k * n * esize(dtype) * div_up(m, few_block(m)) / 3.5e6);
+    return (f32)(5 + (double)k * n * esize(dtype) * div_up(m, few_block(m)) / 7e6);
 }
 
 static int few(u32 m, u32 k, u32 n, u32 dtype, GemmArgs a) {
     const u32 mr = few_block(m);
-    /* A W that is read in a few us has narrow strips of columns and K whole:
-     * joining splits takes 4 us. A longer one has wide strips and about 512
-     * workgroups, two on each compute unit. */
-    const int narrow = k <= FEW_CHUNK && (u64)k * n * esize(dtype) <= FEW_NARROW;
-    const u32 cols = (narrow ? 64 : 256) / (u32)esize(dtype);
+    /* wide strips: a workgroup a compute unit (two, of one row of 16-bit values) */
+    const int narrow = few_narrow(m, k, n, dtype);
+    const u32 cols = (narrow ? 64 : 256) / (u32)esize(dtype), full = mr == 1 && dtype == DTYPE_F16 ? 512 : 256;
     const u64 strips = div_up(n, cols), blocks = div_up(m, mr);
-    u64 splits = narrow || !few_fits(m, FEW_CHUNK + 1, n, dtype) ? 1 : 512 / (strips * blocks);
+    u64 splits = narrow || !few_fits(m, FEW_CHUNK + 1, n, dtype) ? 1 : full / (strips * blocks);
     if (splits < 1) splits = 1;
-    u64 per = round_up(div_up(k ? k : 1, splits), narrow ? 256 : 128);
+    u64 per = round_up(div_up(k ? k : 1, splits), 256);
     if (per > FEW_CHUNK) per = FEW_CHUNK;
     a.kper = (u32)per;
     a.splits = (u32)div_up(k ? k : 1, per);
@@ -473,6 +489,7 @@ int thvm_hip_linear(u32 y, u32 z, u32 x, u32 w, u32 bias, u32 res, u32 act, u32 
     if (act >= ACT_COUNT) return refuse(op, "an unknown activation");
     if (!y || !x || !w) return refuse(op, "no input, weights or output");
     if (k > MAX_SUM) return refuse(op, "sums of more than 2^24 products");
+    if (m > MAX_SIDE || n > MAX_SIDE) return refuse(op, "more than 2^28 rows or columns");
     const u64 es = esize(dtype), mn = (u64)m * n * es;
     const Operand o[] = {{y, mn, 1}, {z, mn, 1}, {x, (u64)m * k * es, 0}, {w, (u64)k * n * es, 0}, {bias, n * es, 0}, {res, mn, 0}};
     const u32 same[][2] = {{0, 5}};
@@ -485,12 +502,16 @@ int thvm_hip_linear(u32 y, u32 z, u32 x, u32 w, u32 bias, u32 res, u32 act, u32 
     const Plan pl = plan_of(m, n, k, dtype, 1, 0);
     /* packing takes a launch and the operands' bytes twice over (f32: two launches, three times) */
     const f32 packed = pl.time + (dtype == DTYPE_F16 ? 6 : 12) + (f32)((double)k * (m + (double)n) * 10 / 4e6);
-    if (!k || (few_fits(m, k, n, dtype) && (m <= 16 || (m <= 64 && few_time(m, k, n, dtype) < packed)))) {
+    const int as_is = lies_well(k, dtype) && lies_well(n, dtype);
+    /* as they lie, 16-bit matrices take 4.4 to 13 us for up to 64 rows; narrow strips
+     * are faster than that (64 x 1024 x 1024: 6.5 us, 8.2), wide ones are not, but
+     * for one row (4096 x 4096: 11.3, 12; 64 rows 38, 13) */
+    const int fast = m <= 1 || (as_is ? few_narrow(m, k, n, dtype) : few_time(m, k, n, dtype) < packed);
+    if (!k || (few_fits(m, k, n, dtype) && fast)) {
         operands_ready(o, 6);
         a.A = addr(x); a.B = addr(w);
         rc = few(m, k, n, dtype, a);
     } else {
-        const int as_is = lies_well(k, dtype) && lies_well(n, dtype);
         Packed px = packed_of(m, k, pl.T), pw = packed_of(n, k, pl.T);
         Source src[2] = {{addr(x), 0, 0, m, k, &px, NULL, 0}, {addr(w), 0, 0, k, n, NULL, &pw, 0}};
         u64 part = 0;
@@ -526,6 +547,7 @@ int thvm_hip_linear_grad(u32 dx, u32 dw, u32 db, u32 dy, u32 z, u32 x, u32 w, u3
     if (!dy || (act && !z) || (dx && !w) || (dw && !x)) return refuse(op, "no gradient, input or weights, or no values before the activation");
     if (!dx && !dw && !db) return refuse(op, "no output");
     if ((dx && n > MAX_SUM) || (dw && m > MAX_SUM)) return refuse(op, "sums of more than 2^24 products");
+    if (m > MAX_SIDE || k > MAX_SIDE || n > MAX_SIDE) return refuse(op, "more than 2^28 rows or columns");
     const u64 es = esize(dtype), mn = (u64)m * n * es;
     const Operand o[] = {{dx, (u64)m * k * es, 1}, {dw, (u64)k * n * es, 1}, {db, n * es, 1}, {dy, mn, 0},
                          {act ? z : 0, mn, 0}, {dw ? x : 0, (u64)m * k * es, 0}, {dx ? w : 0, (u64)k * n * es, 0}};

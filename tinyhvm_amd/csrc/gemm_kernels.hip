@@ -971,11 +971,12 @@ __device__ __forceinline__ void sum_parts(const glob<float> *part, glob<T> *out,
 // the wave's 4 rows of W as well.
 template <typename T, u32 MR, u32 BYTES>
 __device__ __forceinline__ void few_rows(const GemmArgs &a) {
-    constexpr u32 N = BYTES / sizeof(T), U = BYTES == 4 ? 8 : 4, WAVES = 8, KSTEP = WAVES * 4, COLS = 16 * N, OUT = MR * COLS;
-    constexpr u32 PITCH = FEW_CHUNK + 4;     // of 16 rows and 4 k a wave reads 64 banks
-    __shared__ float lds[MR * PITCH > WAVES * OUT ? MR * PITCH : WAVES * OUT];
+    constexpr u32 N = BYTES / sizeof(T), WAVES = 8, COLS = 16 * N, OUT = MR * COLS;
+    constexpr u32 PITCH = FEW_CHUNK + 4;
+    constexpr u32 XS = MR == 16 ? 0 : MR * PITCH;
+    __shared__ float lds[XS > WAVES * OUT ? XS : WAVES * OUT];
     const u32 lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    const u32 kr = wave * 4 + (lane >> 4), c = blockIdx.x * COLS + (lane & 15u) * N;
+    const u32 c = blockIdx.x * COLS + (lane & 15u) * N;
     const u32 per = a.kper, k0 = blockIdx.y * per, k1 = k0 + per < a.K ? k0 + per : a.K;
     const u32 m0 = blockIdx.z * MR, rows = a.M - m0 < MR ? a.M - m0 : MR;
     const glob<T> *W = (const glob<T> *)a.B, *X = (const glob<T> *)a.A + (u64)m0 * a.K;
@@ -985,63 +986,108 @@ __device__ __forceinline__ void few_rows(const GemmArgs &a) {
     for (u32 j = 0; j < N; j++)
 #pragma unroll
         for (u32 r = 0; r < R; r++) acc[j][r] = 0.0f;
-    // past the end W is taken as 0, and x too
-    any_vec<T, N> w[2][U];
-    auto ask = [&](u32 kb, any_vec<T, N> (&v)[U]) {
+    // Loads have no conditions, which would part them: a lane past the last
+    // columns reads the last there are, one past the last k
+    // reads that, and takes 0.
+    const u32 cc = c + N <= a.N ? c : a.N < N ? 0u : a.N - N;
+    auto row = [&](u32 k) { return *(const glob<any_vec<T, N>> *)(W + (u64)(k < k1 ? k : k1 - 1) * a.N + cc); };
+    if constexpr (MR == 16) {
+        // units of 128 k; what is left of them is asked for first, and added last
+        constexpr u32 D = BYTES == 4 ? 8 : 4;
+        const u32 units = (k1 - k0) / 128, kr = wave * 16 + (lane >> 4) * 4, kt = k0 + units * 128 + kr;
+        const glob<T> *xr = X + (u64)((lane & 15u) < rows ? lane & 15u : rows - 1) * a.K;
+        any_vec<T, 4> x[D], xt;
+        any_vec<T, N> w[D][4], wt[4];
+        auto ask = [&](u32 u, any_vec<T, 4> &xv, any_vec<T, N> (&v)[4]) {
+            const u32 k = k0 + u * 128 + kr;
+            xv = *(const glob<any_vec<T, 4>> *)(xr + k);
 #pragma unroll
-        for (u32 u = 0; u < U; u++) {
-            const u32 k = kb + u * KSTEP + kr;
-            if (k < k1 && c + N <= a.N) v[u] = *(const glob<any_vec<T, N>> *)(W + (u64)k * a.N + c);
-            else
+            for (u32 i = 0; i < 4; i++) v[i] = *(const glob<any_vec<T, N>> *)(W + (u64)(k + i) * a.N + cc);
+        };
+        auto multiply = [&](any_vec<T, 4> xv, const any_vec<T, N> (&v)[4]) {
 #pragma unroll
-                for (u32 j = 0; j < N; j++) v[u][j] = k < k1 && c + j < a.N ? W[(u64)k * a.N + c + j] : (T)0.0f;
-        }
-    };
-    auto multiply = [&](u32 kb, const any_vec<T, N> (&v)[U]) {
-#pragma unroll
-        for (u32 u = 0; u < U; u++) {
-            const float *x = lds + kb - k0 + u * KSTEP + kr;
-            if constexpr (MR == 16) {
-                const float xv = x[(lane & 15u) * PITCH];
+            for (u32 i = 0; i < 4; i++)
 #pragma unroll
                 for (u32 j = 0; j < N; j++) {
                     f4 t = {acc[j][0], acc[j][1], acc[j][2], acc[j][3]};
-                    t = __builtin_amdgcn_mfma_f32_16x16x4f32(xv, (float)v[u][j], t, 0, 0, 0);
+                    t = __builtin_amdgcn_mfma_f32_16x16x4f32((float)xv[i], (float)v[i][j], t, 0, 0, 0);
                     acc[j][0] = t[0], acc[j][1] = t[1], acc[j][2] = t[2], acc[j][3] = t[3];
                 }
-            } else {
+        };
+        const bool rest = (k1 - k0) % 128 != 0;
+        if (rest) {
+#pragma unroll
+            for (u32 i = 0; i < 4; i++) xt[i] = xr[kt + i < k1 ? kt + i : k1 - 1], wt[i] = row(kt + i);
+        }
+        if (units) {
+#pragma unroll
+            for (u32 d = 0; d < D; d++) ask(d < units ? d : units - 1, x[d], w[d]);
+            for (u32 u = 0; u < units; u += D)
+#pragma unroll
+                for (u32 d = 0; d < D; d++) {
+                    if (u + d < units) multiply(x[d], w[d]);
+                    if (u + D < units) ask(u + D + d < units ? u + D + d : units - 1, x[d], w[d]);
+                }
+        }
+        if (rest) {
+#pragma unroll
+            for (u32 i = 0; i < 4; i++) {
+                xt[i] = kt + i < k1 ? xt[i] : (T)0.0f;
+#pragma unroll
+                for (u32 j = 0; j < N; j++) wt[i][j] = kt + i < k1 ? wt[i][j] : (T)0.0f;
+            }
+            multiply(xt, wt);
+        }
+    } else if (k0 < k1) {
+        constexpr u32 U = BYTES == 4 ? 8 : 4, KSTEP = WAVES * 4;
+        const u32 kr = wave * 4 + (lane >> 4);
+        any_vec<T, N> w[2][U];
+        auto ask = [&](u32 kb, any_vec<T, N> (&v)[U]) {
+#pragma unroll
+            for (u32 u = 0; u < U; u++) v[u] = row(kb + u * KSTEP + kr);
+        };
+        auto multiply = [&](u32 kb, const any_vec<T, N> (&v)[U]) {
+#pragma unroll
+            for (u32 u = 0; u < U; u++) {
+                const u32 k = kb + u * KSTEP + kr;
+                const float *x = lds + k - k0;
+                any_vec<T, N> t = v[u];
+#pragma unroll
+                for (u32 j = 0; j < N; j++) t[j] = k < k1 ? t[j] : (T)0.0f;
 #pragma unroll
                 for (u32 r = 0; r < MR; r++)
 #pragma unroll
-                    for (u32 j = 0; j < N; j++) acc[j][r] = fmaf(x[r * PITCH], (float)v[u][j], acc[j][r]);
+                    for (u32 j = 0; j < N; j++) acc[j][r] = fmaf(x[r * PITCH], (float)t[j], acc[j][r]);
             }
-        }
-    };
-    ask(k0, w[0]);
+        };
+        ask(k0, w[0]);
 #pragma unroll
-    for (u32 r = 0; r < MR; r++)
-        for (u32 k = threadIdx.x; k < per; k += 512) lds[r * PITCH + k] = r < rows && k0 + k < k1 ? (float)X[(u64)r * a.K + k0 + k] : 0.0f;
-    __syncthreads();
-    // per is a multiple of U * KSTEP
-    for (u32 kb = k0; kb < k0 + per; kb += 2 * U * KSTEP) {
-        ask(kb + U * KSTEP, w[1]);
-        multiply(kb, w[0]);
-        if (kb + U * KSTEP >= k0 + per) break;
-        ask(kb + 2 * U * KSTEP, w[0]);
-        multiply(kb + U * KSTEP, w[1]);
+        for (u32 r = 0; r < MR; r++)
+            for (u32 k = threadIdx.x; k < per; k += 512) lds[r * PITCH + k] = r < rows && k0 + k < k1 ? (float)X[(u64)r * a.K + k0 + k] : 0.0f;
+        __syncthreads();
+        // per is a multiple of U * KSTEP
+        for (u32 kb = k0; kb < k0 + per; kb += 2 * U * KSTEP) {
+            ask(kb + U * KSTEP, w[1]);
+            multiply(kb, w[0]);
+            if (kb + U * KSTEP >= k0 + per) break;
+            ask(kb + 2 * U * KSTEP, w[0]);
+            multiply(kb + U * KSTEP, w[1]);
+        }
+        __syncthreads();
     }
-    __syncthreads();
     // the waves' sums, in order
 #pragma unroll
     for (u32 r = 0; r < R; r++)
 #pragma unroll
         for (u32 j = 0; j < N; j++) {
-            if constexpr (MR == 16) lds[wave * OUT + ((lane >> 4) * 4 + r) * COLS + (lane & 15u) * N + j] = acc[j][r];
-            else {
+            const u32 at = cc + j - blockIdx.x * COLS;      // a lane's own columns only
+            if constexpr (MR == 16) {
+                if (cc + j >= c) lds[wave * OUT + ((lane >> 4) * 4 + r) * COLS + at] = acc[j][r];
+            } else {
                 float s = acc[j][r];
                 s += __shfl_xor(s, 16);
                 s += __shfl_xor(s, 32);
-                if (lane < 16) lds[wave * OUT + r * COLS + lane * N + j] = s;
+                if (lane < 16 && cc + j >= c) lds[wave * OUT + r * COLS + at] = s;
             }
         }
     __syncthreads();
@@ -1134,17 +1180,16 @@ NS(64x64, f32, float)
         pack_tile<PL, T, true>(a, &m, blockIdx.x);                                                                              \
     }                                                                                                              \
     extern "C" __global__ __launch_bounds__(256) void thvm_muon_momentum_##name(MuonArgs m) { muon_momentum<T>(m); } \
-    extern "C" __global__ __launch_bounds__(1024) void thvm_sum_parts_##name(u64 part, u64 out, u32 C, u32 parts) { \
-        sum_parts<T>((const glob<float> *)part, (glob<T> *)out, C, parts);                                                      \
-    }                                                                                                              \
     extern "C" __global__ __launch_bounds__(512) void thvm_few1_##name(GemmArgs a) { few_rows<T, 1, 16>(a); }       \
-    extern "C" __global__ __launch_bounds__(512) void thvm_few4_##name(GemmArgs a) { few_rows<T, 4, 16>(a); }       \
     extern "C" __global__ __launch_bounds__(512) void thvm_few16_##name(GemmArgs a) { few_rows<T, 16, 16>(a); }     \
     extern "C" __global__ __launch_bounds__(512) void thvm_few1n_##name(GemmArgs a) { few_rows<T, 1, 4>(a); }       \
-    extern "C" __global__ __launch_bounds__(512) void thvm_few4n_##name(GemmArgs a) { few_rows<T, 4, 4>(a); }       \
     extern "C" __global__ __launch_bounds__(512) void thvm_few16n_##name(GemmArgs a) { few_rows<T, 16, 4>(a); }
 PER_TYPE(1, f16, f16)
 PER_TYPE(2, f32, float)
+// of 16-bit operands; 32-bit ones' parts are few, and added where they are packed
+extern "C" __global__ __launch_bounds__(1024) void thvm_sum_parts_f16(u64 part, u64 out, u32 C, u32 parts) {
+    sum_parts<f16>((const glob<float> *)part, (glob<f16> *)out, C, parts);
+}
 // of 32-bit operands: 16-bit ones are packed as they are
 extern "C" __global__ __launch_bounds__(512, 4) void thvm_pack_sizes_f32(PackSet s) {
     const u32 i = pack_of(s, blockIdx.x);

@@ -344,8 +344,8 @@ __device__ __forceinline__ void ln_cols(const LnGradArgs &a) {
         ln_bwd<T, G, NV>(a);                                                                                        \
     }
 #define LN_ALL(T)                                                                                                  \
-    LN_KERNELS(T, 64, 1) LN_KERNELS(T, 64, 2) LN_KERNELS(T, 64, 4) LN_KERNELS(T, 64, 8)                            \
-    LN_KERNELS(T, 256, 1) LN_KERNELS(T, 256, 2) LN_KERNELS(T, 256, 4) LN_KERNELS(T, 256, 8)                        \
+    LN_KERNELS(T, 64, 1) LN_KERNELS(T, 64, 2) LN_KERNELS(T, 64, 4)                                                 \
+    LN_KERNELS(T, 256, 1) LN_KERNELS(T, 256, 2) LN_KERNELS(T, 256, 4)                                              \
     LN_KERNELS(T, 1024, 1) LN_KERNELS(T, 1024, 2) LN_KERNELS(T, 1024, 4)                                          \
     extern "C" __global__ __launch_bounds__(1024) void thvm_ln_##T##_long(LnArgs a) { ln_fwd_long<T>(a); }         \
     extern "C" __global__ __launch_bounds__(1024) void thvm_lnb_##T##_long(LnGradArgs a) { ln_bwd_long<T>(a); }    \
@@ -354,6 +354,6 @@ __device__ __forceinline__ void ln_cols(const LnGradArgs &a) {
 LN_ALL(f32)
 LN_ALL(f16)
 LNB_KERNELS(f32, 64, 1) LNB_KERNELS(f32, 64, 2) LNB_KERNELS(f32, 64, 4)
-LNB_KERNELS(f32, 256, 2) LNB_KERNELS(f32, 256, 4) LNB_KERNELS(f32, 512, 2) LNB_KERNELS(f32, 512, 4) LNB_KERNELS(f32, 512, 8)
+LNB_KERNELS(f32, 256, 2) LNB_KERNELS(f32, 512, 2) LNB_KERNELS(f32, 512, 4) LNB_KERNELS(f32, 512, 8)
 LNB_KERNELS(f16, 64, 1) LNB_KERNELS(f16, 64, 2)
-LNB_KERNELS(f16, 256, 1) LNB_KERNELS(f16, 256, 2) LNB_KERNELS(f16, 512, 1) LNB_KERNELS(f16, 512, 2) LNB_KERNELS(f16, 512, 4)
+LNB_KERNELS(f16, 256, 1) LNB_KERNELS(f16, 512, 1) LNB_KERNELS(f16, 512, 2) LNB_KERNELS(f16, 512, 4)
