@@ -454,9 +454,13 @@ static int few_fits(u32 m, u32 k, u32 n, u32 dtype) {
     return div_up(n, 256 / esize(dtype)) * div_up(m, few_block(m)) <= COUNTS || k <= FEW_CHUNK;
 }
 
-/* Its time in us, roughly: W's bytes once a block of rows. */
+/* Its time in us, roughly: W's bytes once a block of rows, or 3.8 a workgroup
+ * that a compute unit takes. */
 static f32 few_time(u32 m, u32 k, u32 n, u32 dtype) {
-    return (f32)(5 + (double)k * n * esize(dtype) * div_up(m, few_block(m)) / 7e6);
+    const u64 blocks = div_up(m, few_block(m));
+    const f32 bytes = (f32)(3.5 + (double)k * n * esize(dtype) * blocks / 7.3e6);
+    const f32 wgs = (f32)(3.8 / 256 * div_up(n, (few_narrow(m, k, n, dtype) ? 64 : 256) / esize(dtype)) * blocks);
+    return bytes > wgs ? bytes : wgs;
 }
 
 static int few(u32 m, u32 k, u32 n, u32 dtype, GemmArgs a) {
@@ -482,6 +486,35 @@ static int few(u32 m, u32 k, u32 n, u32 dtype, GemmArgs a) {
     return launch1(name, strips, a.splits, (u32)blocks, 512, &a);
 }
 
+/* 32-bit matrices as they lie, in tiles of 64 (direct_tile in gemm_kernels.hip):
+ * K splits, and the time in us: 1.04 per 64 of K with a workgroup on a compute
+ * unit, 40 % more with several. Of 64 x 4096 x 4096 27 us (few rows: 50; packed:
+ * 63), 128 x 4096 x 4096 44 (91; 68), 256 x 4096 x 4096 75 (174; 81), but of
+ * 64 x 1024 x 4096 15 (9.7; 29) and of 512 x 4096 x 4096 193 (340; 106). */
+static u32 direct_splits(u32 M, u32 N, u32 K, f32 *time) {
+    const u64 tiles = div_up(M, 64) * div_up(N, 64);
+    const f32 units = (f32)div_up(K, 64);
+    u32 best = 1;
+    for (u32 s = 1; s <= 16; s *= 2) {
+        if (s > 1 && (tiles > COUNTS || units / s < 4)) break;
+        const u64 rounds = div_up(tiles * s, hipb.n_cu ? hipb.n_cu : 256);
+        const f32 t = 3 + (f32)rounds * (5 + units / s * 1.04f) * (rounds > 1 ? 1.4f : 1) + (s > 1 ? 2.5f : 0);
+        if (s > 1 && t >= *time) continue;
+        *time = t;
+        best = s;
+    }
+    return best;
+}
+
+static int direct(u32 M, u32 N, u32 K, u32 splits, u64 part, GemmArgs a) {
+    a.M = M; a.N = N; a.K = K;
+    a.tm = (u32)div_up(M, 64); a.tn = (u32)div_up(N, 64);
+    a.kper = (u32)round_up(div_up(K, splits), 64);
+    a.splits = (u32)div_up(K, a.kper);
+    a.part = part; a.count = B.counts;
+    return launch1("thvm_direct_f32", (u64)a.tm * a.tn, a.splits, 1, 256, &a);
+}
+
 int thvm_hip_linear(u32 y, u32 z, u32 x, u32 w, u32 bias, u32 res, u32 act, u32 m, u32 k, u32 n, u32 dtype) {
     if (!hipb.initialized) return THVM_HIP_EINVAL;
     const char *op = "linear";
@@ -501,16 +534,26 @@ int thvm_hip_linear(u32 y, u32 z, u32 x, u32 w, u32 bias, u32 res, u32 act, u32 
     int rc;
     const Plan pl = plan_of(m, n, k, dtype, 1, 0);
     /* packing takes a launch and the operands' bytes twice over (f32: two launches, three times) */
-    const f32 packed = pl.time + (dtype == DTYPE_F16 ? 6 : 12) + (f32)((double)k * (m + (double)n) * 10 / 4e6);
+    const f32 packed = pl.time + (dtype == DTYPE_F16 ? 6 : 12) + (f32)((double)k * (m + (double)n) * 10 / 4.8e6);
     const int as_is = lies_well(k, dtype) && lies_well(n, dtype);
+    f32 straight;
+    const u32 splits = direct_splits(m, n, k, &straight);
     /* as they lie, 16-bit matrices take 4.4 to 13 us for up to 64 rows; narrow strips
      * are faster than that (64 x 1024 x 1024: 6.5 us, 8.2), wide ones are not, but
      * for one row (4096 x 4096: 11.3, 12; 64 rows 38, 13) */
-    const int fast = m <= 1 || (as_is ? few_narrow(m, k, n, dtype) : few_time(m, k, n, dtype) < packed);
+    const f32 rows_time = few_time(m, k, n, dtype);
+    const int fast = m <= 1 || (as_is ? few_narrow(m, k, n, dtype) : rows_time < packed && (dtype != DTYPE_F32 || rows_time < straight));
     if (!k || (few_fits(m, k, n, dtype) && fast)) {
         operands_ready(o, 6);
         a.A = addr(x); a.B = addr(w);
         rc = few(m, k, n, dtype, a);
+    } else if (dtype == DTYPE_F32 && n > 1 && straight < packed) {
+        Carve c = {0, 0};
+        carve(&c, splits > 1 ? 16384ull * splits * div_up(m, 64) * div_up(n, 64) : 0);
+        if (!carve_reserve(&c)) return THVM_HIP_ENOMEM;
+        operands_ready(o, 6);
+        a.A = addr(x); a.B = addr(w);
+        rc = direct(m, n, k, splits, carve(&c, 0), a);
     } else {
         Packed px = packed_of(m, k, pl.T), pw = packed_of(n, k, pl.T);
         Source src[2] = {{addr(x), 0, 0, m, k, &px, NULL, 0}, {addr(w), 0, 0, k, n, NULL, &pw, 0}};

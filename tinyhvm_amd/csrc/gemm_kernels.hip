@@ -1135,6 +1135,153 @@ __device__ __forceinline__ void few_rows(const GemmArgs &a) {
     }
 }
 
+// ---- 32-bit products of matrices as they lie ----
+
+// A 64 x 64 tile on the 32-bit matrix instruction (v_mfma_f32_32x32x2_f32, 64
+// multiplications a cycle and compute unit where the planes' three products
+// reach some 340), for sizes at which packing would take longer than that
+// costs. The 4 waves of a workgroup take 16 k of 64 each and add their sums at
+// the end, so nothing passes through LDS on the way in and no wave waits for
+// another. Of those 16 k lane half h holds k = 8 h .. + 7: of x 8 of two rows,
+// in 16-byte loads, of W two neighbouring columns at each of the 8 k. D such
+// units are on their way. 128 x 4096 x 4096: 44 us, 98 TFLOP/s of the 150 that
+// the instruction gives.
+struct Direct {
+    static constexpr u32 PITCH = 68, LDS = 4 * 64 * PITCH, D = 2;
+};
+
+// 8 k of two rows of x from k on, or of two columns of W. Past the last row or
+// column a lane reads the last ones.
+__device__ __forceinline__ void direct_x(const glob<float> *const (&row)[2], u32 k, float (&v)[2][8]) {
+#pragma unroll
+    for (u32 i = 0; i < 2; i++)
+#pragma unroll
+        for (u32 q = 0; q < 2; q++) {
+            const any_vec<float, 4> x = *(const glob<any_vec<float, 4>> *)(row[i] + k + q * 4);
+#pragma unroll
+            for (u32 j = 0; j < 4; j++) v[i][q * 4 + j] = x[j];
+        }
+}
+__device__ __forceinline__ void direct_w(const glob<float> *col, u64 ld, u32 k, float (&v)[2][8]) {
+#pragma unroll
+    for (u32 j = 0; j < 8; j++) {
+        const any_vec<float, 2> x = *(const glob<any_vec<float, 2>> *)(col + (k + j) * ld);
+        v[0][j] = x[0], v[1][j] = x[1];
+    }
+}
+
+__device__ __forceinline__ void direct_tile(const GemmArgs &a, float *lds) {
+    constexpr u32 D = Direct::D, PITCH = Direct::PITCH;
+    const u32 lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    u32 ti, tj;
+    tile_of(blockIdx.x, a.tm, a.tn, ti, tj);
+    const u32 k0 = blockIdx.y * a.kper, k1 = k0 + a.kper < a.K ? k0 + a.kper : a.K;
+    const u32 units = k0 < k1 ? (k1 - k0) / 64 : 0, kr = wave * 16 + (lane >> 5) * 8, kt = k0 + units * 64 + kr;
+    const bool rest = k0 < k1 && (k1 - k0) % 64 != 0;
+    const glob<float> *row[2];
+#pragma unroll
+    for (u32 i = 0; i < 2; i++) {
+        const u32 r = ti * 64 + i * 32 + (lane & 31u);
+        row[i] = (const glob<float> *)a.A + (u64)(r < a.M ? r : a.M - 1) * a.K;
+    }
+    const u32 own = tj * 64 + (lane & 31u) * 2, at = own + 2 <= a.N ? own : a.N - 2;
+    const glob<float> *col = (const glob<float> *)a.B + at;
+    f16v acc[2][2];
+#pragma unroll
+    for (u32 i = 0; i < 2; i++)
+#pragma unroll
+        for (u32 j = 0; j < 2; j++) acc[i][j] = 0.0f;
+    float x[D][2][8], w[D][2][8], xt[2][8], wt[2][8];
+    auto multiply = [&](const float (&xv)[2][8], const float (&wv)[2][8]) {
+#pragma unroll
+        for (u32 k = 0; k < 8; k++)
+#pragma unroll
+            for (u32 i = 0; i < 2; i++)
+#pragma unroll
+                for (u32 j = 0; j < 2; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(xv[i][k], wv[j][k], acc[i][j], 0, 0, 0);
+    };
+    // what is left of the units is asked for first, and added last
+    if (rest)
+#pragma unroll
+        for (u32 j = 0; j < 8; j++) {
+            const u32 k = kt + j < k1 ? kt + j : k1 - 1;
+            const any_vec<float, 2> v = *(const glob<any_vec<float, 2>> *)(col + (u64)k * a.N);
+            xt[0][j] = row[0][k], xt[1][j] = row[1][k], wt[0][j] = v[0], wt[1][j] = v[1];
+        }
+    if (units) {
+#pragma unroll
+        for (u32 d = 0; d < D; d++) {
+            const u32 k = k0 + (d < units ? d : units - 1) * 64 + kr;
+            direct_x(row, k, x[d]), direct_w(col, a.N, k, w[d]);
+        }
+        for (u32 u = 0; u < units; u += D)
+#pragma unroll
+            for (u32 d = 0; d < D; d++) {
+                if (u + d < units) multiply(x[d], w[d]);
+                const u32 k = k0 + (u + D + d < units ? u + D + d : units - 1) * 64 + kr;
+                direct_x(row, k, x[d]), direct_w(col, a.N, k, w[d]);
+            }
+    }
+    if (rest) {
+#pragma unroll
+        for (u32 j = 0; j < 8; j++)
+            if (kt + j >= k1) xt[0][j] = xt[1][j] = wt[0][j] = wt[1][j] = 0.0f;
+        multiply(xt, wt);
+    }
+    // the waves' sums, in order: a lane has rows v / 4 * 8 + h * 4 + v % 4 of its columns
+    float *st = lds + wave * (64 * PITCH);
+#pragma unroll
+    for (u32 i = 0; i < 2; i++)
+#pragma unroll
+        for (u32 v = 0; v < 16; v++)
+#pragma unroll
+            for (u32 j = 0; j < 2; j++)
+                if (at + j >= own) st[(i * 32 + (v >> 2) * 8 + (lane >> 5) * 4 + (v & 3)) * PITCH + at + j - tj * 64] = acc[i][j][v];
+    __syncthreads();
+    const u32 dc = (threadIdx.x & 15u) * 4, dr = threadIdx.x >> 4, c = tj * 64 + dc, r0 = ti * 64 + dr;
+    f4 sum[4];
+#pragma unroll
+    for (u32 q = 0; q < 4; q++) {
+        const float *row = lds + (dr + q * 16) * PITCH + dc;
+        sum[q] = *(const f4 *)row;
+#pragma unroll
+        for (u32 k = 1; k < 4; k++) sum[q] += *(const f4 *)(row + k * 64 * PITCH);
+    }
+    if (a.splits > 1) {
+        const u64 base = a.part + (u64)blockIdx.x * a.splits * 16384u;
+#pragma unroll
+        for (u32 q = 0; q < 4; q++) put_part(base + blockIdx.y * 16384u, threadIdx.x * 16u + q * 4096u, sum[q]);
+        if (!last_of(a.count + blockIdx.x * 4ull, a.splits)) return;
+#pragma unroll
+        for (u32 q = 0; q < 4; q++) sum[q] = f4{0, 0, 0, 0};
+#pragma unroll 4
+        for (u32 s = 0; s < a.splits; s++)
+#pragma unroll
+            for (u32 q = 0; q < 4; q++) sum[q] += get_part(base + s * 16384u, threadIdx.x * 16u + q * 4096u);
+    }
+    if (c >= a.N) return;
+    float bias[4] = {0, 0, 0, 0}, res[4][4];
+    if (a.bias) load_n<float, 4>((const glob<float> *)a.bias, c, a.N, bias);
+    if (a.res)
+#pragma unroll
+        for (u32 q = 0; q < 4; q++)
+            if (r0 + q * 16 < a.M) load_n<float, 4>((const glob<float> *)a.res + (u64)(r0 + q * 16) * a.N, c, a.N, res[q]);
+#pragma unroll
+    for (u32 q = 0; q < 4; q++) {
+        const u32 r = r0 + q * 16;
+        if (r >= a.M) break;
+        float v[4];
+#pragma unroll
+        for (u32 j = 0; j < 4; j++) v[j] = sum[q][j] + bias[j];
+        if (a.z) store_n<float, 4>((glob<float> *)a.z + (u64)r * a.N, c, a.N, v);
+        act_n<4>(a.act, v);
+        if (a.res)
+#pragma unroll
+            for (u32 j = 0; j < 4; j++) v[j] += res[q][j];
+        store_n<float, 4>((glob<float> *)a.out + (u64)r * a.N, c, a.N, v);
+    }
+}
+
 // ---- the kernels ----
 
 #define GEMM(size, TILE, name, T, ...)                                                                             \
@@ -1194,4 +1341,8 @@ extern "C" __global__ __launch_bounds__(1024) void thvm_sum_parts_f16(u64 part, 
 extern "C" __global__ __launch_bounds__(512, 4) void thvm_pack_sizes_f32(PackSet s) {
     const u32 i = pack_of(s, blockIdx.x);
     pack_sizes<float>(s.p[i], blockIdx.x - s.first[i]);
+}
+extern "C" __global__ __launch_bounds__(256) void thvm_direct_f32(GemmArgs a) {
+    __shared__ __attribute__((aligned(16))) float lds[Direct::LDS];
+    direct_tile(a, lds);
 }
