@@ -151,7 +151,9 @@ int  thvm_hip_dispatch_uop_kernel_noalloc(u32 out_buf, const u32 *leaf_bufs, u32
  * and products' sums are in 32 bits or more and an output is rounded once, to
  * the nearest. Results are the same bits in every run. An operand may name
  * the same buffer as an output only where it says so. Sizes of 0 are empty
- * tensors, and their sums 0. The calls do not wait; workspaces come from the
+ * tensors, and their sums 0. A sum has at most 2^24 terms (a row of layer
+ * norm, k, the rows of dw, the columns of dx), a side of a linear layer at
+ * most 2^28. The calls do not wait; workspaces come from the
  * pool and stay for the next call. Returns THVM_HIP_OK, or:
  *   THVM_HIP_EINVAL   not initialised, or arguments that cannot be (the reason
  *                     goes to stderr); nothing is launched

@@ -8,7 +8,7 @@ import pytest
 
 from tests import blockops as bo
 from tests.blockops import F16, F32, NP, U32
-from tests.test_gpu_block import _grad_check, _linear_check, _linear_inputs, _muon_inputs, within
+from tests.test_gpu_block import _grad_check, _linear_check, _linear_inputs, _ln_check, _ln_inputs, _muon_inputs, within
 
 pytestmark = pytest.mark.gpu
 
@@ -50,6 +50,14 @@ def test_16_bit_layer_infinities_and_nan(hip):
     fin = np.isfinite(want)
     # 88 products of values under 5 and 1 in 32 bits, and one rounding to 16
     assert np.all(np.abs(got[fin] - want[fin]) <= 92 * U32 * 88 * 5 + 2.0 ** -11 * np.abs(want[fin]) + 2.0 ** -25)
+
+
+@pytest.mark.parametrize("dt", [F32, F16], ids=["f32", "f16"])
+@pytest.mark.parametrize("rows,cols", [(600, 4096), (515, 4099), (4100, 1000), (4099, 1999), (1500, 1000), (1025, 500), (511, 4096)], ids=str)
+def test_layer_norm_rows(hip, rows, cols, dt):
+    """Rows enough for a wave, or a small workgroup, to take longer ones."""
+    _, x, gamma, beta = _ln_inputs(rows, cols, dt, rows + cols)
+    _ln_check(hip, x, gamma, beta, 1e-5, dt)
 
 
 # few rows in narrow strips and wide ones, K whole, split and with an end of its own; two rows to hundreds

@@ -1,9 +1,14 @@
-// gemm_kernels.hip - matrix products on the 16-bit matrix instructions, with
-// the epilogues of a linear layer, of its gradients and of the Newton-Schulz
+// gemm_kernels.hip - matrix products on the matrix instructions, with the
+// epilogues of a linear layer, of its gradients and of the Newton-Schulz
 // step (thvm_hip_linear, thvm_hip_linear_grad, thvm_hip_muon_step).
 //
-// Operands. Every product is C[r][c] = sum_k A[r][k] B[c][k] of two packed
-// operands. Packing lays an operand out as the matrix instruction
+// Three kinds, of which block.c takes the one that its estimate puts first:
+// tiles on the 16-bit instruction over packed operands or 16-bit matrices as
+// they lie, the bulk of this file; 64 x 64 tiles on the 32-bit instruction over
+// 32-bit matrices as they lie (direct_tile), of up to a few hundred rows; and
+// few rows (few_rows), which read W once.
+//
+// Packed operands. A product is C[r][c] = sum_k A[r][k] B[c][k]. Packing lays an operand out as the matrix instruction
 // (v_mfma_f32_32x32x16_f16) takes it: blocks of 32 rows by 16 k, 1 KB each,
 // lane l's 16 bytes being k = 8 (l / 32) .. + 7 of row l % 32. A block goes
 // from memory to LDS as it is (one 16-byte load a lane that writes LDS
@@ -21,6 +26,12 @@
 // A row that holds an infinity or NaN is marked, and its outputs are
 // computed again by plain 32-bit sums over the planes (exact_dot).
 // 16-bit operands are one plane as they are.
+//
+// What bounds the large tiles is power: of 4096^3 in 16 bits 137 us, 1003
+// TFLOP/s (a library product 1155 on the same card), as they lie; packed ones
+// alone 129. In 32 bits 310 to 330 us, 1250 to 1330 TFLOP/s of 16-bit products,
+// at which the card holds its clock near 1.6 GHz with the matrix units busy 74 %
+// of the cycles. Small ones are bound by the latency of one stage after another.
 #include <hip/hip_runtime.h>
 #include "thvm_abi.h"
 #include "block_args.h"
@@ -956,19 +967,22 @@ __device__ __forceinline__ void sum_parts(const glob<float> *part, glob<T> *out,
 
 // ---- few rows ----
 
-// y = x W, MR rows a workgroup (blockIdx.z). W is read once, as it lies
-// ([K][N] row-major), BYTES a lane, 16 lanes along a row and the workgroup's
-// 8 waves 32 rows at a time. Bound by W's bytes where W is large: 16 bytes a
-// lane, and K split over workgroups (blockIdx.y) until the card is full. Bound
-// by latency where it is small: 4 bytes a lane, which makes four times the
-// workgroups without a split to join. U of a lane's loads are on their way
-// while U are multiplied; a split's part of x lies in LDS from the start, so
-// that the loop has no barrier.
+// y = x W, MR rows a workgroup (blockIdx.z). W is read once a block of rows, as
+// it lies ([K][N] row-major), BYTES a lane, 16 lanes along a row. Bound by W's
+// bytes where W is large: 16 bytes a lane, and K split over workgroups
+// (blockIdx.y) until the card is full (1 x 4096 x 4096 f16: 11.3 us, 3 TB/s with
+// the launch and the join). Bound by latency where it is small: 4 bytes a lane,
+// which makes four times the workgroups without a split to join (1 x 1024 x
+// 1024 f32 3.8 us against 5.6, 64 x 784 x 128 5.2).
 //
-// Products are 32-bit ones, of 1 or 4 rows on the vector unit, of 16 on the
-// 32-bit matrix instruction (v_mfma_f32_16x16x4_f32: lane l holds k = l / 16
-// of row, or column, l % 16), one for each of a lane's columns; it adds up
-// the wave's 4 rows of W as well.
+// Products are 32-bit ones. One row: on the vector unit, the workgroup's 8 waves
+// 32 rows of W at a time, U of a lane's loads on their way while U are
+// multiplied, the split's part of x in LDS from the start. 16 rows: on the
+// 32-bit matrix instruction (v_mfma_f32_16x16x4_f32: lane l holds k = l / 16 of
+// row, or column, l % 16), one for each of a lane's columns and k. A wave takes
+// 16 k of a unit of 128, lane group q its k = 4 q .. + 3, so that x too comes
+// from memory in vectors of 4 k and neither LDS nor a barrier stands ahead of
+// the sums; D units are on their way.
 template <typename T, u32 MR, u32 BYTES>
 __device__ __forceinline__ void few_rows(const GemmArgs &a) {
     constexpr u32 N = BYTES / sizeof(T), WAVES = 8, COLS = 16 * N, OUT = MR * COLS;
