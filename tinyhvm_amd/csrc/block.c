@@ -304,16 +304,19 @@ typedef struct { u32 T, tm, tn, splits, lanes; f32 time; const char *name; u32 t
  * workgroups. What each takes, in us, as measured on products of 512 to 4096
  * rows and columns over K of 512 to 8192: `unit` per 16 of K (f16, f32; with
  * every compute unit at work), `fixed` for the launch, the first loads and the
- * epilogue, `join0 + join1 * splits` for joining K splits. */
+ * epilogue, `join + per_join * splits` and the parts' bytes at `rate` for joining
+ * K splits (optimiser steps in f32: 784 x 128, whose first product has 3 tiles,
+ * 93 us with 4 splits, 97 with 2, 102 with none; 768 x 768, 78 tiles, 172 with 2,
+ * 163 with none). */
 static const struct {
     u32 T, lanes, slots;      /* slots: workgroups a compute unit holds, which then share its time */
     const char *name;
-    f32 unit[2], fixed[2], join;
+    f32 unit[2], fixed[2], join, per_join, rate;
 } TILES[] = {
-    {256, 512, 1, "256x256", {0.41f, 1.15f}, {10, 18}, 15},
-    {192, 256, 1, "192x192", {0.27f, 0.75f}, {8, 12}, 10},     /* of a symmetric product only */
-    {128, 256, 1, "128x128", {0.13f, 0.335f}, {6, 9}, 5},
-    {64, 256, 2, "64x64", {0.055f, 0.11f}, {5, 6}, 3},
+    {256, 512, 1, "256x256", {0.41f, 1.15f}, {10, 18}, 15, 1, 3e6f},
+    {192, 256, 1, "192x192", {0.27f, 0.75f}, {8, 12}, 10, 1, 3e6f},     /* of a symmetric product only */
+    {128, 256, 1, "128x128", {0.13f, 0.335f}, {6, 9}, 5, 1, 3e6f},
+    {64, 256, 2, "64x64", {0.055f, 0.11f}, {5, 6}, 1, 0.25f, 1.3e6f},
 };
 #define TILE_SYM 1
 
@@ -330,12 +333,12 @@ static Plan plan_of(u32 M, u32 N, u32 K, u32 dtype, u32 count, int sym) {
         const u32 tm = (u32)div_up(M, TILES[i].T), tn = (u32)div_up(N, TILES[i].T);
         const u64 tiles = sym ? (u64)tm * (tm + 1) / 2 : (u64)tm * tn;
         for (u32 s = 1; s <= 16; s *= 2) {
-            if (s > 1 && (tiles * count > COUNTS || units / s < 16)) break;
+            if (s > 1 && (tiles * count > COUNTS || units / s < 12)) break;
             const u64 wgs = tiles * count * s, rounds = div_up(wgs, (u64)cu * TILES[i].slots);
             /* two workgroups of a compute unit take 1.9 times one's time */
             const f32 share = TILES[i].slots == 2 && wgs > cu ? 1.9f * (f32)rounds : (f32)rounds;
             const f32 t = TILES[i].fixed[f] + share * units / s * TILES[i].unit[f] +
-                          (s > 1 ? TILES[i].join + s + (f32)wgs * TILES[i].T * TILES[i].T * 4 / 3e6f : 0);
+                          (s > 1 ? TILES[i].join + TILES[i].per_join * s + (f32)wgs * TILES[i].T * TILES[i].T * 4 / TILES[i].rate : 0);
             if (best.T && t >= best.time) continue;
             best = (Plan){TILES[i].T, tm, tn, s, TILES[i].lanes, t, TILES[i].name, (u32)tiles};
         }
