@@ -27,11 +27,11 @@
 // computed again by plain 32-bit sums over the planes (exact_dot).
 // 16-bit operands are one plane as they are.
 //
-// What bounds the large tiles is power: of 4096^3 in 16 bits 137 us, 1003
-// TFLOP/s (a library product 1155 on the same card), as they lie; packed ones
-// alone 129. In 32 bits 310 to 330 us, 1250 to 1330 TFLOP/s of 16-bit products,
-// at which the card holds its clock near 1.6 GHz with the matrix units busy 74 %
-// of the cycles. Small ones are bound by the latency of one stage after another.
+// Large tiles: of 4096^3 in 16 bits as they lie 135 us, 1018 TFLOP/s (a library
+// product 1155 on the same card; packed ones alone 129 us), the matrix units
+// busy 55 % of the cycles with one read of LDS a product; in 32 bits 318 us,
+// 1297 TFLOP/s of 16-bit products, busy 73 %. Either way the card holds its clock
+// near 1.7 GHz. Small ones are bound by the latency of one stage after another.
 #include <hip/hip_runtime.h>
 #include "thvm_abi.h"
 #include "block_args.h"
