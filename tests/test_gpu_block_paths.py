@@ -138,6 +138,26 @@ def test_linear_past_32_bits(hip):
             del got
 
 
+@pytest.mark.parametrize("k", [0, 1024])
+def test_more_rows_than_a_launch_counts(hip, k):
+    """Few columns, in blocks of 16 rows, of which a launch has 65535."""
+    L, m, n, period = hip, 65535 * 16 + 37, 2, 101
+    rng = np.random.default_rng(6)
+    x, w = rng.standard_normal((period, k)).astype(np.float16), (rng.standard_normal((k, n)) / 32).astype(np.float16)
+    res = rng.standard_normal((period, n)).astype(np.float16)
+    bias = rng.standard_normal(n).astype(np.float16)
+    at = np.arange(m) % period
+    z64 = x.astype(np.float64) @ w.astype(np.float64) + bias.astype(np.float64)
+    mag = np.abs(x.astype(np.float64)) @ np.abs(w.astype(np.float64)) + np.abs(bias.astype(np.float64))
+    with bo.Bufs(L) as b:
+        y, z = b.out((m, n), np.float16), b.out((m, n), np.float16)
+        assert L.thvm_hip_linear(y, z, b.put(x[at]), b.put(w), b.put(bias), b.put(res[at]), 1, m, k, n, F16) == 0
+        bound = (k + 4) * U32 * mag
+        within(b.get(z), z64[at], (bound + bo.rounding(F16, z64))[at])
+        want = np.maximum(z64, 0) + res.astype(np.float64)
+        within(b.get(y), want[at], (bound + U32 * np.abs(want) + bo.rounding(F16, want))[at])
+
+
 def test_layer_norm_past_32_bits(hip):
     L, cols, period = hip, 65544, 97
     rows = 33000

@@ -484,7 +484,7 @@ static int few(u32 m, u32 k, u32 n, u32 dtype, GemmArgs a) {
     if (per > FEW_CHUNK) per = FEW_CHUNK;
     a.kper = (u32)per;
     a.splits = (u32)div_up(k ? k : 1, per);
-    a.M = m; a.N = n; a.K = k;
+    a.N = n; a.K = k;
     Carve c = {0, 0};
     carve(&c, a.splits > 1 ? 4ull * a.splits * strips * cols * blocks * mr : 0);
     if (!carve_reserve(&c)) return THVM_HIP_ENOMEM;
@@ -492,7 +492,19 @@ static int few(u32 m, u32 k, u32 n, u32 dtype, GemmArgs a) {
     a.count = B.counts;
     char name[48];
     snprintf(name, sizeof name, "thvm_few%u%s_%s", mr, narrow ? "n" : "", tname(dtype));
-    return launch1(name, strips, a.splits, (u32)blocks, 512, &a);
+    /* a launch counts 65535 blocks of rows */
+    int rc = THVM_HIP_OK;
+    const u64 es = esize(dtype), step = 65535ull * mr;
+    for (u64 r0 = 0; r0 < m && !rc; r0 += step) {
+        GemmArgs p = a;
+        p.M = (u32)(m - r0 < step ? m - r0 : step);
+        p.A += r0 * k * es;
+        p.out += r0 * n * es;
+        if (p.z) p.z += r0 * n * es;
+        if (p.res) p.res += r0 * n * es;
+        rc = launch1(name, strips, a.splits, (u32)div_up(p.M, mr), 512, &p);
+    }
+    return rc;
 }
 
 /* 32-bit matrices as they lie, in tiles of 64 (direct_tile in gemm_kernels.hip):
