@@ -11,10 +11,11 @@
 // is that of the centred values, so a large mean costs no bits. 16-bit
 // values are rounded once, on the way out.
 //
-// Measured: forward 8192 x 4096 f32 49 us, 268 MB at 5.5 TB/s (a large copy
-// takes 54 us for as many); 8 x 4096 f16 3 us, a launch and two memory
-// latencies. Backward 8192 x 4096 f16 with what is added, 270 MB, 52 us and
-// 4.8 us for the column sums; 4097 x 1000 f32 13.5 and 4 us.
+// Measured: forward 8192 x 4096 f32 49 to 51 us in a row of calls, 268 MB at 5.4
+// TB/s (a large copy takes 54 us for as many), 42 us on inputs that lie in the
+// last-level cache in part; 8 x 4096 f16 3.7 us, a launch and two memory
+// latencies. Backward 8192 x 4096 f16 with what is added, 270 MB, 51 us and 4.8
+// us for the column sums; 4097 x 1000 f32 14.5 and 3.9 us.
 #include <hip/hip_runtime.h>
 #include "thvm_abi.h"
 #include "block_args.h"
