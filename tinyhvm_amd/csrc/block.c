@@ -196,11 +196,11 @@ int thvm_hip_layer_norm(u32 y, u32 mean, u32 rstd, u32 x, u32 gamma, u32 beta, u
     else snprintf(name, sizeof name, "thvm_ln_%s_long", tname(dtype)), g = 1024;
     int rc = THVM_HIP_OK;
     /* a launch holds fewer than 2^32 lanes */
-    for (u32 r0 = 0, step = (1u << 31) / g; r0 < rows && !rc; r0 += step) {
-        const u32 nr = rows - r0 < step ? rows - r0 : step;
-        const u64 off = (u64)r0 * v;
-        LnArgs a = {addr(x) + off, addr(gamma), addr(beta), addr(y) + off, mean ? addr(mean) + r0 * 4ull : 0,
-                    rstd ? addr(rstd) + r0 * 4ull : 0, nr, cols, eps, 0};
+    for (u64 r0 = 0, step = (1u << 31) / g; r0 < rows && !rc; r0 += step) {
+        const u32 nr = (u32)(rows - r0 < step ? rows - r0 : step);
+        const u64 off = r0 * v;
+        LnArgs a = {addr(x) + off, addr(gamma), addr(beta), addr(y) + off, mean ? addr(mean) + r0 * 4 : 0,
+                    rstd ? addr(rstd) + r0 * 4 : 0, nr, cols, eps, 0};
         rc = launch1(name, g < 256 ? div_up(nr, 256 / g) : nr, 1, 1, g < 256 ? 256 : g, &a);
     }
     operands_written(o, 6);
@@ -253,13 +253,13 @@ int thvm_hip_layer_norm_grad(u32 dx, u32 dgamma, u32 dbeta, u32 dy, u32 x, u32 m
             rc = launch1(name, div_up(cols, 256), parts, 1, 256, &a);
         }
         snprintf(name, sizeof name, "thvm_lnb_%s_long", tname(dtype));
-        for (u32 r0 = 0, step = 1u << 21; dx && r0 < rows && !rc; r0 += step) {
-            const u64 off = (u64)r0 * v;
+        for (u64 r0 = 0, step = 1u << 21; dx && r0 < rows && !rc; r0 += step) {
+            const u64 off = r0 * v;
             LnGradArgs b = a;
-            b.rows = rows - r0 < step ? rows - r0 : step;
+            b.rows = (u32)(rows - r0 < step ? rows - r0 : step);
             b.dy += off; b.x += off; b.dx += off;
             if (b.add) b.add += off;
-            b.mean += r0 * 4ull; b.rstd += r0 * 4ull;
+            b.mean += r0 * 4; b.rstd += r0 * 4;
             rc = launch1(name, b.rows, 1, 1, 1024, &b);
         }
     }
