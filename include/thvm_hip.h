@@ -166,7 +166,8 @@ int  thvm_hip_dispatch_uop_kernel_noalloc(u32 out_buf, const u32 *leaf_bufs, u32
 #define THVM_HIP_ACT_SILU 4       /* z / (1 + exp -z) */
 /* Layer norm of the rows of x [rows][cols]: y = (x - mean) * rstd * gamma +
  * beta, rstd = 1 / sqrt(variance + eps). gamma and beta [cols] may be absent
- * (1 and 0); mean and rstd [rows] f32 are kept where given. y may be x. */
+ * (1 and 0); mean and rstd [rows] f32 are kept where given, NaN of rows of no
+ * columns. y may be x. */
 int  thvm_hip_layer_norm(u32 y, u32 mean, u32 rstd, u32 x, u32 gamma, u32 beta, u32 rows, u32 cols, f32 eps, u32 dtype);
 /* Its gradient from dy, x and the kept mean and rstd: dx [rows][cols], with
  * `add` (0: nothing) added, the gradient that reaches x past the

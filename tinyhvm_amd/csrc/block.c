@@ -187,7 +187,7 @@ int thvm_hip_layer_norm(u32 y, u32 mean, u32 rstd, u32 x, u32 gamma, u32 beta, u
     const Operand o[] = {{y, n, 1}, {mean, st, 1}, {rstd, st, 1}, {x, n, 0}, {gamma, v, 0}, {beta, v, 0}};
     const u32 same[][2] = {{0, 3}};
     if (!operands_ok(op, o, 6, same, 1)) return THVM_HIP_EINVAL;
-    if (!rows || !cols) return THVM_HIP_OK;
+    if (!rows || (!cols && !mean && !rstd)) return THVM_HIP_OK;
     operands_ready(o, 6);
     u32 g, nv;
     char name[48];
