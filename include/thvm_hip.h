@@ -160,7 +160,7 @@ int  thvm_hip_dispatch_uop_kernel_noalloc(u32 out_buf, const u32 *leaf_bufs, u32
  *   THVM_HIP_ENOMEM   no memory for the workspace; nothing is launched
  *   THVM_HIP_EDEVICE  a launch failed; outputs are undefined */
 #define THVM_HIP_ACT_NONE 0
-#define THVM_HIP_ACT_RELU 1
+#define THVM_HIP_ACT_RELU 1       /* z, 0 below 0; NaN stays NaN, here and in act' */
 #define THVM_HIP_ACT_GELU 2       /* z (1 + erf(z / sqrt 2)) / 2 */
 #define THVM_HIP_ACT_GELU_TANH 3  /* its tanh form */
 #define THVM_HIP_ACT_SILU 4       /* z / (1 + exp -z) */

@@ -34,3 +34,61 @@ def test_statistics_of_empty_rows(hip, rows, dt):
         x = b.put(np.zeros((rows, 0), NP[dt]))
         assert hip.thvm_hip_layer_norm(b.out((rows, 0), NP[dt]), m, r, x, 0, 0, rows, 0, 1e-5, dt) == 0
         assert np.isnan(b.get(m)).all() and np.isnan(b.get(r)).all()
+
+
+# ---- NaN and infinities through an activation ----
+
+# a layer's kernels: few rows, 32-bit tiles as they lie, packed, 16-bit as they lie
+KERNELS = [((1, 40, 60), F32, "thvm_few1n_f32"), ((20, 40, 60), F32, "thvm_few16n_f32"), ((500, 60, 2000), F32, "thvm_direct_f32"),
+           ((2100, 70, 1900), F32, "thvm_gemm_64x64_f32"), ((1, 40, 60), F16, "thvm_few1n_f16"), ((200, 1192, 264), F16, "thvm_gemm_rc_64x64_f16"),
+           ((2100, 70, 1900), F16, "thvm_gemm_64x64_f16")]
+
+
+def _layer(shape, dt):
+    m, k, n = shape
+    rng = np.random.default_rng(m + n)
+    return rng, rng.standard_normal((m, k)).astype(NP[dt]), (rng.standard_normal((k, n)) / math.sqrt(k)).astype(NP[dt])
+
+
+@pytest.mark.parametrize("name", ACTS)
+@pytest.mark.parametrize("shape,dt,kernel", KERNELS, ids=str)
+def test_nan_stays(hip, shape, dt, kernel, name):
+    """A row that diverged does not come out healthy, and spoils no other."""
+    got = bp.linear(*shape, dt)[-1]
+    assert got == kernel
+    _, x, w = _layer(shape, dt)
+    m = shape[0]
+    clean, _ = bo.run_linear(hip, x, w, None, None, name, dt)
+    x[m // 2, 7] = np.nan
+    y, z = bo.run_linear(hip, x, w, None, None, name, dt)
+    assert np.isnan(z[m // 2]).all() and np.isnan(y[m // 2]).all()
+    keep = np.arange(m) != m // 2
+    assert np.array_equal(y[keep], clean[keep])
+
+
+@pytest.mark.parametrize("name", ACTS)
+@pytest.mark.parametrize("dt", [F32, F16], ids=["f32", "f16"])
+def test_nan_stays_in_gradients(hip, dt, name):
+    """From dy and from the kept values: in its row of dx, its column of dw
+    and of db."""
+    m, k, n = 70, 50, 90
+    rng, x, w = _layer((m, k, n), dt)
+    dy, z = rng.standard_normal((2, m, n)).astype(NP[dt])
+    for where in ("dy", "z") if name != "none" else ("dy",):
+        a = {"dy": dy.copy(), "z": z.copy()}
+        a[where][9, 11] = np.nan
+        dx, dw, db = bo.run_linear_grad(hip, a["dy"], a["z"], x, w, name, dt)
+        assert np.isnan(dx[9]).all() and np.isnan(dw[:, 11]).all() and np.isnan(db[11])
+
+
+@pytest.mark.parametrize("name", ACTS)
+@pytest.mark.parametrize("dt", [F32, F16], ids=["f32", "f16"])
+def test_infinities_through_an_activation(hip, dt, name):
+    """Up, every activation is its argument; down, relu's is 0 and the others'
+    formulas are a product of 0 and infinity."""
+    bias = np.array([np.inf, -np.inf, 1.0, -1.0], NP[dt])
+    y, z = bo.run_linear(hip, np.zeros((3, 0), NP[dt]), np.zeros((0, 4), NP[dt]), bias, None, name, dt)
+    assert np.array_equal(z, np.broadcast_to(bias, z.shape))
+    assert np.all(y[:, 0] == np.inf) and np.isfinite(y[:, 2:]).all()
+    low = {"none": -np.inf, "relu": 0.0}.get(name, np.nan)
+    assert np.array_equal(y[:, 1], np.full(3, low, NP[dt]), equal_nan=True)

@@ -65,7 +65,7 @@ __device__ __forceinline__ float normal_cdf(float z) {
 
 __device__ __forceinline__ float act_of(u32 act, float z) {
     switch (act) {
-    case ACT_RELU: return z > 0.0f ? z : 0.0f;
+    case ACT_RELU: return z <= 0.0f ? 0.0f : z;      // NaN stays
     case ACT_GELU: return z * normal_cdf(z);
     case ACT_GELU_TANH: return z * sigmoid(GELU_U * (z + GELU_C * z * z * z));
     case ACT_SILU: return z * sigmoid(z);
@@ -78,7 +78,7 @@ __device__ __forceinline__ float act_of(u32 act, float z) {
 __device__ __forceinline__ float act_slope(u32 act, float z) {
     const float near = fminf(fmaxf(z, -128.0f), 128.0f);
     switch (act) {
-    case ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
+    case ACT_RELU: return z > 0.0f ? 1.0f : z <= 0.0f ? 0.0f : z;
     case ACT_GELU: return normal_cdf(z) + near * (0.3989422804014327f * __expf(-0.5f * near * near));
     case ACT_GELU_TANH: {
         const float s = sigmoid(GELU_U * (z + GELU_C * z * z * z));
