@@ -35,6 +35,13 @@ def _view(rows, cols, stride=None):
     return v
 
 
+def shape_factor(inputs, outputs):
+    """The published factor of an orthogonalised update (K. Jordan et al.,
+    "Muon", 2024): sqrt(max(1, outputs / inputs)). Matrices lie here as
+    [inputs][outputs]."""
+    return math.sqrt(max(1.0, outputs / inputs))
+
+
 class ResidualBlock:
     """The block's buffers and its calls, for `rows` inputs at a time."""
 
@@ -107,7 +114,7 @@ class ResidualBlock:
         for name in self.MATRICES:
             rows, cols = self.shapes[name]
             self._done(L.thvm_hip_muon_step(_one(b[name]), _one(b["d" + name]), _one(b["m" + name]), 1, rows, cols, lr,
-                                            math.sqrt(max(1.0, rows / cols)), 0.0, 0.95, 1, 5, F32))
+                                            shape_factor(rows, cols), 0.0, 0.95, 1, 5, F32))
         for name in self.VECTORS:
             L.thvm_hip_adam_step(b[name], b["d" + name], b["m" + name], b["v" + name], lr_vectors, 0.9, 0.99, 1e-8,
                                  1 - 0.9 ** step, 1 - 0.99 ** step, self.shapes[name][0])
