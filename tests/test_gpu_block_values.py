@@ -74,11 +74,14 @@ def test_nan_stays_in_gradients(hip, dt, name):
     m, k, n = 70, 50, 90
     rng, x, w = _layer((m, k, n), dt)
     dy, z = rng.standard_normal((2, m, n)).astype(NP[dt])
+    clean = bo.run_linear_grad(hip, dy, z, x, w, name, dt)
     for where in ("dy", "z") if name != "none" else ("dy",):
         a = {"dy": dy.copy(), "z": z.copy()}
         a[where][9, 11] = np.nan
         dx, dw, db = bo.run_linear_grad(hip, a["dy"], a["z"], x, w, name, dt)
         assert np.isnan(dx[9]).all() and np.isnan(dw[:, 11]).all() and np.isnan(db[11])
+        assert np.array_equal(np.delete(dx, 9, 0), np.delete(clean[0], 9, 0))
+        assert np.array_equal(np.delete(dw, 11, 1), np.delete(clean[1], 11, 1)) and np.array_equal(np.delete(db, 11), np.delete(clean[2], 11))
 
 
 @pytest.mark.parametrize("name", ACTS)

@@ -349,7 +349,8 @@ static Plan plan_of(u32 M, u32 N, u32 K, u32 dtype, u32 count, int sym) {
 static u64 plan_part_bytes(const Plan *p) { return p->splits > 1 ? 4ull * p->tiles * p->splits * p->T * p->T : 0; }
 
 /* The product of two operands with its epilogue (a: out, z, bias, res, act).
- * `lie`: A is [M][K] and B [K][N] as they lie, else both are packed. */
+ * `lie`: A is [M][K] and B [K][N] as they lie, else both are packed (a.oa and
+ * a.ob: from what). */
 static int product(const Plan *pl, int lie, const Packed *pa, const Packed *pb, u32 M, u32 N, u32 K, u32 dtype, u64 part,
                    GemmArgs a) {
     char name[48];
@@ -595,6 +596,8 @@ int thvm_hip_linear(u32 y, u32 z, u32 x, u32 w, u32 bias, u32 res, u32 act, u32 
             a.lda = k; a.ldb = n;
             rc = product(&pl, 1, &px, &pw, m, n, k, dtype, part, a);
         } else {
+            a.oa = (Origin){addr(x), 0, k, 1, 0, 0};
+            a.ob = (Origin){addr(w), 0, 1, n, 0, 0};
             rc = pack(src, 2, dtype);
             if (!rc) rc = product(&pl, 0, &px, &pw, m, n, k, dtype, part, a);
         }
@@ -644,10 +647,14 @@ int thvm_hip_linear_grad(u32 dx, u32 dw, u32 db, u32 dy, u32 z, u32 x, u32 w, u3
     int rc = pack(src, ns, dtype);
     if (dx && !rc) {
         a.out = addr(dx);
+        a.oa = (Origin){addr(dy), act ? addr(z) : 0, n, 1, act, 0};
+        a.ob = (Origin){addr(w), 0, n, 1, 0, 0};
         rc = product(&px_, 0, &zr, &wr, m, k, n, dtype, part, a);
     }
     if (dw && !rc) {
         a.out = addr(dw);
+        a.oa = (Origin){addr(x), 0, 1, k, 0, 0};
+        a.ob = (Origin){addr(dy), act ? addr(z) : 0, 1, n, act, 0};
         rc = product(&pw_, 0, &xc, &zc, k, n, m, dtype, part, a);
     }
     operands_written(o, 7);

@@ -28,10 +28,18 @@ enum { ACT_NONE = 0, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU, ACT_COUNT };
 /* bytes past a packed operand that a product's last loads may touch */
 #define PACK_SLACK 32768
 
+/* An operand as the caller has it: value k of row r is p[r * row + k * step]
+ * (in elements; one of the two steps is 1), times act'(z) there if z is given */
+typedef struct {
+    u64 p, z;
+    u32 row, step, act, pad;
+} Origin;
+
 /* C[M][N] = sum over k of A[r][k] B[c][k], packed operands (gemm_kernels.hip) */
 typedef struct {
     u64 A, B;                  /* packed; KB blocks of 16 k */
-    u64 ea, eb;                /* exponent words of A's and B's rows (32-bit operands) */
+    u64 ea, eb;                /* exponents of A's and B's rows (32-bit operands) */
+    Origin oa, ob;             /* what the packed operands were */
     u64 out, z, bias, res;     /* row-major [M][N]; bias [N] */
     u64 part, count;           /* the K splits' sums, and how many of a tile's are there (0 between launches) */
     u32 M, N, KB, tm, tn, splits, act;
@@ -46,8 +54,8 @@ typedef struct {
 typedef struct {
     u64 src, z;                /* z 0: the matrix itself */
     u64 pn, pt;                /* packed with rows r (Rn of them, KBn blocks of k = c); with rows c */
-    u64 en, et;                /* their exponent words */
-    u64 row_part, col_part;    /* size words [row_parts][R], [col_parts][C] */
+    u64 en, et;                /* their exponents */
+    u64 row_part, col_part;    /* the largest magnitudes' bits [row_parts][R], [col_parts][C] */
     u64 sum_part;              /* column sums [..][C] f32 */
     u64 stride;                /* bytes between the matrices of a batch in pn and pt */
     u32 R, C, act, rt;         /* rt: rows of a column part */

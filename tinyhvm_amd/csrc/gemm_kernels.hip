@@ -23,8 +23,10 @@
 // row's largest. Of the four products three are summed, hi hi + hi lo +
 // lo hi; lo lo is at most 2^-24 of the product. All sums are 32 bits. So a
 // 32-bit product costs three 16-bit ones, where three bf16 planes cost six.
-// A row that holds an infinity or NaN is marked, and its outputs are
-// computed again by plain 32-bit sums over the planes (exact_dot).
+// A sum that is not finite, as each is that an infinity or NaN goes into, is
+// computed again from the operands as the caller has them, in 32-bit sums of
+// 32-bit products (block_again): of 4096^3 with a NaN in every row 2.0 ms, in one
+// row 0.72, in none 0.42.
 // 16-bit operands are one plane as they are.
 //
 // Large tiles: of 4096^3 in 16 bits as they lie 135 us, 1018 TFLOP/s (a library
@@ -121,27 +123,6 @@ __device__ __forceinline__ void split(float v, f16 &hi, f16 &lo) {
     hi = (f16)v;
     const float h = (float)hi;
     lo = fabsf(h) < __builtin_inff() ? (f16)(v - h) : (f16)0.0f;
-}
-
-// A row's exponent word: e, and whether the row holds an infinity or NaN.
-#define EXP_MARK 0x40000000
-__device__ __forceinline__ int exp_of(int w) { return (w << 2) >> 2; }
-__device__ __forceinline__ bool exp_marked(int w) { return ((w >> 30) & 1) != ((w >> 31) & 1); }
-
-// The sum of a row's products with the planes as they are, in 32 bits.
-template <u32 PL>
-__device__ __forceinline__ float exact_dot(const glob<f16> *A, const glob<f16> *B, u32 KB, u32 r, u32 c) {
-    float s = 0.0f;
-    for (u32 kb = 0; kb < KB; kb++)
-        for (u32 t = 0; t < 16; t++) {
-            const u32 at = (t >> 3) * 256u + (t & 7u);
-            const u64 ia = block_at<PL>(r >> 5, kb, KB, 0) + at + (r & 31u) * 8u;
-            const u64 ib = block_at<PL>(c >> 5, kb, KB, 0) + at + (c & 31u) * 8u;
-            float a = (float)A[ia], b = (float)B[ib];
-            if (PL == 2) a += (float)A[ia + 512], b += (float)B[ib + 512];
-            s = fmaf(a, b, s);
-        }
-    return s;
 }
 
 // ---- the product ----
@@ -373,6 +354,61 @@ __device__ __forceinline__ void stage_rows(float *st, const f16v (&acc)[TL::NI])
     __builtin_amdgcn_wave_barrier();
 }
 
+// ---- outputs computed again ----
+
+// Values k .. k + 15 of row r of an operand as the caller has it, zeros from
+// `end` on. Loads have no conditions, which would part them: past the end they
+// read the last value.
+template <typename T>
+__device__ __forceinline__ void origin16(const Origin &o, u32 r, u32 k, u32 end, float (&v)[16]) {
+    const glob<T> *p = (const glob<T> *)o.p + (u64)r * o.row, *z = (const glob<T> *)o.z + (u64)r * o.row;
+    const bool whole = k + 16 <= end;
+    float at[16];
+    auto each = [&](const glob<T> *from, float (&to)[16]) {
+        if (o.step == 1 && whole) {
+#pragma unroll
+            for (u32 j = 0; j < 16; j += 4) {
+                const any_vec<T, 4> q = *(const glob<any_vec<T, 4>> *)(from + k + j);
+#pragma unroll
+                for (u32 i = 0; i < 4; i++) to[j + i] = (float)q[i];
+            }
+        } else
+#pragma unroll
+            for (u32 j = 0; j < 16; j++) to[j] = (float)from[(u64)(k + j < end ? k + j : end - 1) * o.step];
+    };
+    each(p, v);
+    if (o.z) {
+        each(z, at);
+        slope_n<16>(o.act, at, v);
+    }
+    if (!whole)
+#pragma unroll
+        for (u32 j = 0; j < 16; j++) v[j] = k + j < end ? v[j] : 0.0f;
+}
+
+// A 32 x 32 block of the product from the operands as the caller has them, on
+// the 32-bit matrix instruction, by one wave: what 32-bit sums of 32-bit
+// products make of infinities and NaN. Of 32 k lane half h holds k = 16 h .. +
+// 15; they are asked for while the 32 before are multiplied.
+template <typename T>
+__device__ __forceinline__ f16v block_again(const GemmArgs &a, u32 rb, u32 cb) {
+    const u32 lane = threadIdx.x & 63u, h = (lane >> 5) * 16, r = rb + (lane & 31u), c = cb + (lane & 31u);
+    const u32 ra = r < a.M ? r : a.M - 1, rc = c < a.N ? c : a.N - 1;
+    f16v acc = 0.0f;
+    float x[16] = {}, w[16] = {}, x1[16], w1[16];
+    if (!a.K) return acc;
+#pragma unroll 1
+    for (u32 k = 0; k < a.K + 32; k += 32) {
+        origin16<T>(a.oa, ra, k + h, a.K, x1);
+        origin16<T>(a.ob, rc, k + h, a.K, w1);
+#pragma unroll
+        for (u32 j = 0; j < 16; j++) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j], w[j], acc, 0, 0, 0);
+#pragma unroll
+        for (u32 j = 0; j < 16; j++) x[j] = x1[j], w[j] = w1[j];
+    }
+    return acc;
+}
+
 // What an output becomes: z = sum (+ bias), y = act(z) (+ residual).
 template <typename T>
 __device__ __forceinline__ void finish1(const GemmArgs &a, u32 r, u32 c, float v) {
@@ -382,25 +418,6 @@ __device__ __forceinline__ void finish1(const GemmArgs &a, u32 r, u32 c, float v
     v = act_of(a.act, v);
     if (a.res) v += (float)((const glob<T> *)a.res)[at];
     ((glob<T> *)a.out)[at] = (T)v;
-}
-
-// One output whose row or column is marked, its sum computed again.
-template <u32 PL, typename T>
-__device__ __forceinline__ void finish_marked(const GemmArgs &a, u32 r, u32 c) {
-    const int e = exp_of(((const glob<int> *)a.ea)[r]) + exp_of(((const glob<int> *)a.eb)[c]);
-    finish1<T>(a, r, c, ldexpf(exact_dot<PL>((const glob<f16> *)a.A, (const glob<f16> *)a.B, a.KB, r, c), -e));
-}
-
-// The exponents of 8 columns (padded to whole tiles), and whether one is marked.
-__device__ __forceinline__ bool column_exps(const GemmArgs &a, u32 c, int *ec) {
-    bool odd = false;
-#pragma unroll
-    for (u32 j = 0; j < 8; j++) {
-        const int w = ((const glob<int> *)a.eb)[c + j];
-        odd |= exp_marked(w);
-        ec[j] = exp_of(w);
-    }
-    return odd;
 }
 
 // The operand of a tile that begins at row r0, from stage s0 on.
@@ -520,9 +537,11 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs &a, f16 *lds) {
     const bool whole = c + 8 <= a.N;
     float bias[8];
     int ec[8];
-    bool odd = false, left = false;      // a column that is marked; outputs left for later
+    u32 later[TL::MI];      // outputs of row block i that are not finished yet: bit 8 p + j
     if (a.bias) load8<T>((const glob<T> *)a.bias, c, a.N, bias);
-    if (TL::PL == 2) odd = column_exps(a, c, ec);
+    if (TL::PL == 2)
+#pragma unroll
+        for (u32 j = 0; j < 8; j++) ec[j] = ((const glob<int> *)a.eb)[c + j];
     any_vec<T, 8> res[2][PASSES];
     auto ask = [&](u32 i, any_vec<T, 8> (&x)[PASSES]) {
 #pragma unroll
@@ -536,6 +555,7 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs &a, f16 *lds) {
     for (u32 i = 0; i < TL::MI; i++) {
         if (i + 1 < TL::MI) ask(i + 1, res[(i + 1) & 1]);
         stage_rows<TL>(st, acc[i]);
+        later[i] = 0;
 #pragma unroll
         for (u32 p = 0; p < PASSES; p++) {
             const u32 r = r0 + i * 32 + p * RPP;
@@ -544,9 +564,18 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs &a, f16 *lds) {
             *(f4 *)v = *(const f4 *)(row + p * RPP * TL::PITCH);
             *(f4 *)(v + 4) = *(const f4 *)(row + p * RPP * TL::PITCH + 4);
             if (TL::PL == 2) {
+                u32 most = 0;
+#pragma unroll
+                for (u32 j = 0; j < 8; j++) most = max(most, __float_as_uint(v[j]) & 0x7FFFFFFFu);
                 const int er = ((const glob<int> *)a.ea)[r];
-                if (odd || exp_marked(er)) {
-                    left = true;
+                if (most >= 0x7F800000u) {
+                    // one by one, those that stand
+#pragma unroll 1
+                    for (u32 j = 0; j < 8 && c + j < a.N; j++) {
+                        const float x = row[p * RPP * TL::PITCH + j];
+                        if (fabsf(x) < __builtin_inff()) finish1<T>(a, r, c + j, ldexpf(x, -(er + ((const glob<int> *)a.eb)[c + j])));
+                        else later[i] |= 1u << (p * 8 + j);
+                    }
                     continue;
                 }
 #pragma unroll
@@ -570,11 +599,28 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs &a, f16 *lds) {
             store8<T>((glob<T> *)a.out + at, c, a.N, v);
         }
     }
-    if (TL::PL == 2 && left)
-        for (u32 q = 0; q < TL::MI * PASSES; q++) {
-            const u32 r = r0 + q * RPP;
-            if (r < a.M && (odd || exp_marked(((const glob<int> *)a.ea)[r])))
-                for (u32 j = 0; j < 8 && c + j < a.N; j++) finish_marked<TL::PL, T>(a, r, c + j);
+    if (TL::PL == 2)
+#pragma unroll 1
+        for (u32 i = 0; i < TL::MI; i++) {
+            u32 mine = later[0];
+#pragma unroll
+            for (u32 q = 1; q < TL::MI; q++) mine = q == i ? later[q] : mine;
+            if (!__ballot(mine != 0)) continue;
+            const u32 rb = ti * TL::TM + ((wave / TL::WN) * TL::MI + i) * 32, cb = tj * TL::TN + (wave % TL::WN) * TL::NI * 32;
+#pragma unroll 1
+            for (u32 j = 0; j < TL::NI; j++) {
+                if (!__ballot(mine != 0 && dc / 32 == j)) continue;
+                const f16v again = block_again<T>(a, rb, cb + j * 32);
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                for (u32 v = 0; v < 16; v++) st[((v >> 2) * 8 + (lane >> 5) * 4 + (v & 3)) * TL::PITCH + j * 32 + (lane & 31u)] = again[v];
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+            for (u32 b = 0; b < PASSES * 8; b++)
+                if ((mine >> b) & 1u) finish1<T>(a, r0 + i * 32 + b / 8 * RPP, c + b % 8, row[b / 8 * RPP * TL::PITCH + b % 8]);
+            __builtin_amdgcn_wave_barrier();
         }
 }
 
@@ -755,20 +801,9 @@ __device__ __forceinline__ void muon_momentum(const MuonArgs &a) {
 
 // ---- packing ----
 
-__device__ __forceinline__ u32 size_word(float v) {
-    const u32 b = __float_as_uint(v) & 0x7FFFFFFFu;
-    return b < 0x7F800000u ? b : 0x80000000u;
-}
-__device__ __forceinline__ u32 size_join(u32 a, u32 b) {
-    const u32 x = a & 0x7FFFFFFFu, y = b & 0x7FFFFFFFu;
-    return (x > y ? x : y) | ((a | b) & 0x80000000u);
-}
-// the exponent word of a row whose largest finite value and mark are w
-__device__ __forceinline__ int exp_word(u32 w) {
-    const float v = __uint_as_float(w & 0x7FFFFFFFu);
-    const int e = v > 0.0f ? 14 - ilogbf(v) : 0;
-    return w & 0x80000000u ? e ^ EXP_MARK : e;
-}
+// the exponent of a row whose largest magnitude's bits are w: of a row with an
+// infinity or NaN, whose products are not finite whatever it is, 0
+__device__ __forceinline__ int exp_of(u32 w) { return w && w < 0x7F800000u ? 14 - ilogbf(__uint_as_float(w)) : 0; }
 
 // The matrix of a set that a workgroup works on.
 __device__ __forceinline__ u32 pack_of(const PackSet &s, u32 block) {
@@ -786,15 +821,14 @@ __device__ __forceinline__ void source(const PackArgs &a, u32 r, u32 c, float *v
     }
 }
 
-// The largest values of a matrix's rows and columns (as size words, a part a
-// column tile of 512 and a row tile of a.rt) and the columns' sums.
-// 8 waves, each every 8th row of the tile, a lane 8 columns; two rows are
-// asked for at a time. Magnitudes compare as their bits do, and infinities and
-// NaN are the largest of all: a tile that holds one is gone through again,
-// with the words that keep the largest finite value beside the mark. Bound by
-// memory: three matrices of 4096 x 4096, one with its act', 63 us, 4.2 TB/s.
-template <typename T, bool MARKS>
-__device__ __forceinline__ bool pack_sizes_of(const PackArgs &a, u32 bx, u32 by, u32 (*lw)[512], float (*ls)[512]) {
+// The largest values of a matrix's rows and columns (as the bits of their
+// magnitudes, which compare as they do, with infinities and NaN the largest of
+// all; a part a column tile of 512 and a row tile of a.rt) and the columns'
+// sums. 8 waves, each every 8th row of the tile, a lane 8 columns; two rows are
+// asked for at a time. Bound by memory: three matrices of 4096 x 4096, one with
+// its act', 63 us, 4.2 TB/s.
+template <typename T>
+__device__ __forceinline__ void pack_sizes_of(const PackArgs &a, u32 bx, u32 by, u32 (*lw)[512], float (*ls)[512]) {
     const u32 lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     const u32 c = bx * 512u + lane * 8u;
     const u64 r0 = (u64)by * a.rt, r1 = r0 + a.rt < a.R ? r0 + a.rt : a.R;
@@ -813,28 +847,20 @@ __device__ __forceinline__ bool pack_sizes_of(const PackArgs &a, u32 bx, u32 by,
             u32 rw = 0;
 #pragma unroll
             for (u32 j = 0; j < 8; j++) {
-                const u32 w = MARKS ? size_word(v[q][j]) : __float_as_uint(v[q][j]) & 0x7FFFFFFFu;
-                rw = MARKS ? size_join(rw, w) : max(rw, w);
-                cw[j] = MARKS ? size_join(cw[j], w) : max(cw[j], w);
+                const u32 w = __float_as_uint(v[q][j]) & 0x7FFFFFFFu;
+                rw = max(rw, w);
+                cw[j] = max(cw[j], w);
                 cs[j] += v[q][j];
             }
             if (a.row_part && r + q * 8 < r1) {
 #pragma unroll
-                for (int d = 32; d; d >>= 1) {
-                    const u32 o = __shfl_xor(rw, d);
-                    rw = MARKS ? size_join(rw, o) : max(rw, o);
-                }
+                for (int d = 32; d; d >>= 1) rw = max(rw, (u32)__shfl_xor(rw, d));
                 if (lane == 0) ((glob<u32> *)a.row_part)[(u64)bx * a.R + r + q * 8] = rw;
             }
         }
     }
-    bool mark = false;
 #pragma unroll
-    for (u32 j = 0; j < 8; j++) {
-        const u32 at = lane * 8 + j;
-        lw[wave][at] = cw[j], ls[wave][at] = cs[j], mark |= cw[j] >= 0x7F800000u;
-    }
-    return mark;
+    for (u32 j = 0; j < 8; j++) lw[wave][lane * 8 + j] = cw[j], ls[wave][lane * 8 + j] = cs[j];
 }
 
 template <typename T>
@@ -842,16 +868,14 @@ __device__ __forceinline__ void pack_sizes(const PackArgs &a, u32 block) {
     __shared__ u32 lw[8][512];
     __shared__ float ls[8][512];
     const u32 bx = block % a.row_parts, by = block / a.row_parts;
-    if (__syncthreads_or(pack_sizes_of<T, false>(a, bx, by, lw, ls))) {
-        pack_sizes_of<T, true>(a, bx, by, lw, ls);
-        __syncthreads();
-    }
+    pack_sizes_of<T>(a, bx, by, lw, ls);
+    __syncthreads();
     const u32 t = threadIdx.x, ct = bx * 512u + t;
     if (ct >= a.C || (!a.col_part && !a.sum_part)) return;
     u32 w = lw[0][t];
     float s = ls[0][t];
 #pragma unroll
-    for (u32 k = 1; k < 8; k++) w = size_join(w, lw[k][t]), s += ls[k][t];
+    for (u32 k = 1; k < 8; k++) w = max(w, lw[k][t]), s += ls[k][t];
     if (a.col_part) ((glob<u32> *)a.col_part)[(u64)by * a.C + ct] = w;
     if (a.sum_part) ((glob<float> *)a.sum_part)[(u64)by * a.C + ct] = s;
 }
@@ -872,16 +896,16 @@ __device__ __forceinline__ void pack_tile(const PackArgs &a, const MuonArgs *mu,
         const u32 i = t >> 2, q = t & 3u;
         u32 wr = 0, wc = 0;
         if (a.pn && r0 + i < a.R)
-            for (u32 p = q; p < a.row_parts; p += 4) wr = size_join(wr, ((const glob<u32> *)a.row_part)[(u64)p * a.R + r0 + i]);
+            for (u32 p = q; p < a.row_parts; p += 4) wr = max(wr, (u32)((const glob<u32> *)a.row_part)[(u64)p * a.R + r0 + i]);
         if (a.pt && c0 + i < a.C)
-            for (u32 p = q; p < a.col_parts; p += 4) wc = size_join(wc, ((const glob<u32> *)a.col_part)[(u64)p * a.C + c0 + i]);
-        wr = size_join(wr, __shfl_xor(wr, 1));
-        wc = size_join(wc, __shfl_xor(wc, 1));
-        wr = size_join(wr, __shfl_xor(wr, 2));
-        wc = size_join(wc, __shfl_xor(wc, 2));
+            for (u32 p = q; p < a.col_parts; p += 4) wc = max(wc, (u32)((const glob<u32> *)a.col_part)[(u64)p * a.C + c0 + i]);
+        wr = max(wr, (u32)__shfl_xor(wr, 1));
+        wc = max(wc, (u32)__shfl_xor(wc, 1));
+        wr = max(wr, (u32)__shfl_xor(wr, 2));
+        wc = max(wc, (u32)__shfl_xor(wc, 2));
         if (q == 0) {
-            er[i] = exp_word(wr);
-            ec[i] = exp_word(wc);
+            er[i] = exp_of(wr);
+            ec[i] = exp_of(wc);
             if (a.pn && c0 == 0 && r0 + i < a.Rn) ((glob<int> *)a.en)[r0 + i] = er[i];
             if (a.pt && r0 == 0 && c0 + i < a.Ct) ((glob<int> *)a.et)[c0 + i] = ec[i];
         }
@@ -929,7 +953,7 @@ __device__ __forceinline__ void pack_tile(const PackArgs &a, const MuonArgs *mu,
         if (a.pn && r < a.Rn && c < a.KBn * 16u) {
             if (PL == 2 && !MUON)
 #pragma unroll
-                for (u32 k = 0; k < 8; k++) v[k] = ldexpf(v[k], exp_of(er[i]));
+                for (u32 k = 0; k < 8; k++) v[k] = ldexpf(v[k], er[i]);
             put_packed<PL>(pn, a.KBn, r, c, v);
         }
     }
@@ -943,7 +967,7 @@ __device__ __forceinline__ void pack_tile(const PackArgs &a, const MuonArgs *mu,
 #pragma unroll
             for (u32 k = 0; k < 8; k++) {
                 v[k] = tile[i + k][j];
-                if (PL == 2 && !MUON) v[k] = ldexpf(v[k], exp_of(ec[j]));
+                if (PL == 2 && !MUON) v[k] = ldexpf(v[k], ec[j]);
             }
             put_packed<PL>(pt, a.KBt, c, r, v);
         }
