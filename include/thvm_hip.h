@@ -177,8 +177,12 @@ int  thvm_hip_layer_norm_grad(u32 dx, u32 dgamma, u32 dbeta, u32 dy, u32 x, u32 
                               u32 rows, u32 cols, u32 dtype);
 /* A linear layer y = act(z) + res, z = x W + bias: x [m][k], W [k][n], bias
  * [n], res, z and y [m][n]. bias and res may be absent; z is kept where
- * given, for the gradient. y may be res. 32-bit products are as exact as
- * 32-bit sums of 32-bit products, infinities and NaN included. */
+ * given, for the gradient. y may be res. A 32-bit sum of K products, here and
+ * in the gradient, is within (2 K + 8) 2^-24 of the sum of their magnitudes,
+ * whatever the operands' range (of products over 2^-126: a smaller one may be
+ * lost); infinities and NaN do what they do in 32-bit sums of 32-bit products.
+ * Rows and columns in which small values decide an output, beside ones 2^16
+ * times as large or more, cost a second computation of it. */
 int  thvm_hip_linear(u32 y, u32 z, u32 x, u32 w, u32 bias, u32 res, u32 act, u32 m, u32 k, u32 n, u32 dtype);
 /* Its gradient from dy and the kept z (not read without an activation): with
  * dz = dy act'(z), dx = dz W^T, dw = x^T dz, db = the column sums of dz. That

@@ -1,8 +1,9 @@
 """32-bit products over the whole range of 32 bits, on every kernel that
-computes them: infinities that meet values far below their row's largest.
+computes them: values far below their row's or column's largest where that one
+is multiplied by 0, and infinities that meet values as small.
 
 A sum of K products is within (2 K + 8) 2^-24 of the sum of the products'
-magnitudes; an output is rounded once more."""
+magnitudes (thvm_hip.h); an output is rounded once more."""
 import numpy as np
 import pytest
 
@@ -34,9 +35,21 @@ def _some(n, count=40):
 
 def _spread(rng, a, b, kind):
     """a [M][K] and b [N][K] (float32, in place) whose product sum_k a b is
-    asked for. broken: an infinity, which meets tiny values and zeros, and a NaN in a,
+    asked for. wide: row 2 of a and rows 3, 5, 7 of b hold one large value
+    beside tiny ones, and meet rows in which the large one's partner is 0.
+    broken: an infinity, which meets tiny values and zeros, and a NaN in a,
     another infinity in b."""
     (m, k), n = a.shape, b.shape[0]
+    if "wide" in kind:
+        a[2] = np.ldexp(a[2], -45)
+        a[2, 0] = 2.0 ** 20
+        b[::2, 0] = 0
+        for r in (3, 5, 7):
+            if r < n and k > 1:
+                b[r] = np.ldexp(b[r], -30)
+                b[r, 1] = 2.0 ** 60
+        a[m // 2:, 1] = 0
+        a[4 % m] = 0                       # a row of zeros stays one
     if "broken" in kind:
         a[m - 1, k - 1], a[m // 2, k // 2] = np.inf, np.nan
         b[n // 2, k - 1], b[n - 1, k - 1] = 1e-13, 0.0
@@ -50,7 +63,7 @@ def _reference(a, b, rows, cols):
         return a64 @ b64.T, np.abs(a64) @ np.abs(b64).T
 
 
-KINDS = ["broken"]
+KINDS = ["wide", "broken", "wide, broken"]
 LAYERS = [((3, 300, 200), "thvm_few16n_f32"), ((17, 2100, 301), "thvm_few16_f32"), ((500, 60, 2000), "thvm_direct_f32"),
           ((130, 4096, 4095), "thvm_direct_f32"), ((700, 5000, 300), "thvm_direct_f32"), ((2100, 70, 1900), "thvm_gemm_64x64_f32"), ((1100, 2000, 1100), "thvm_gemm_64x64_f32"),
           ((1500, 1601, 1499), "thvm_gemm_128x128_f32"), ((8000, 150, 7999), "thvm_gemm_256x256_f32")]
@@ -112,3 +125,82 @@ def test_gradient_of_weights(hip, shape, dx_kernel, dw_kernel, kind):
     want, mag = _reference(x, dy, rows, cols)
     within(dw[rows][:, cols], want, _sum_bound(m, mag, want))
     within(db, dy.astype(np.float64).sum(1), (m + 4) * U32 * np.abs(dy.astype(np.float64)).sum(1) + bo.rounding(F32, dy.astype(np.float64).sum(1)))
+
+
+@pytest.mark.parametrize("name", ["gelu", "silu"])
+@pytest.mark.parametrize("shape", [(50, 60, 70), (300, 130, 260)], ids=str)
+def test_gradient_through_an_activation(hip, shape, name):
+    """What is computed again is dy act'(z), not dy."""
+    m, k, n = shape
+    rng = np.random.default_rng(m + k + n)
+    x, w = rng.standard_normal((m, k)).astype(np.float32), rng.standard_normal((k, n)).astype(np.float32)
+    dy, z = rng.standard_normal((2, m, n)).astype(np.float32)
+    dy[2] = np.ldexp(dy[2], -45)
+    dy[2, 0] = 2.0 ** 20
+    w[::2, 0] = 0
+    dy[:, 5] = np.ldexp(dy[:, 5], -45)
+    dy[3, 5] = 2.0 ** 20
+    x[3, ::2] = 0
+    x[m - 1, 1] = np.inf
+    s = bo.slope(name, z)
+    dz = dy.astype(np.float64) * s
+    edz = np.abs(dy.astype(np.float64)) * (16 * U32 * (1 + np.abs(z.astype(np.float64))))     # act' in 32 bits
+    dx, dw, _ = bo.run_linear_grad(hip, dy, z, x, w, name, F32)
+    w64, x64 = w.astype(np.float64), x.astype(np.float64)
+    want = dz @ w64.T
+    within(dx, want, _sum_bound(n, np.abs(dz) @ np.abs(w64.T), want) + 2 * edz @ np.abs(w64.T))
+    with np.errstate(invalid="ignore"):
+        want = x64.T @ dz
+        within(dw, want, _sum_bound(m, np.abs(x64.T) @ np.abs(dz), want) + 2 * np.abs(x64.T) @ edz)
+
+
+@pytest.mark.parametrize("k", [1, 70, 1000])
+def test_equal_operands(hip, k):
+    """1 + 2^-11 everywhere: what two 16-bit planes leave out has one sign."""
+    m, n = 2100, 1900
+    v = np.float32(1 + 2.0 ** -11)
+    x, w = np.full((m, k), v), np.full((k, n), v)
+    want = np.float64(v) ** 2 * k
+    y, _ = bo.run_linear(hip, x, w, None, None, "none", F32)
+    within(y, np.full((m, n), want), _sum_bound(k, want, want))
+    dx, _, _ = bo.run_linear_grad(hip, np.full((m, n), v), None, None, w, "none", F32, (True, False, False))
+    want = np.float64(v) ** 2 * n
+    within(dx, np.full((m, k), want), _sum_bound(n, want, want))
+
+
+@pytest.mark.parametrize("shape,kernel", [((2100, 300, 1900), "thvm_gemm_64x64_f32"), ((8000, 150, 7999), "thvm_gemm_256x256_f32")], ids=str)
+def test_operands_that_never_meet(hip, shape, kernel):
+    """Faint values whose partners are all 0 leave a sum exactly 0."""
+    m, k, n = shape
+    assert bp.linear(m, k, n, F32)[-1] == kernel
+    rng = np.random.default_rng(k)
+    x, w = rng.standard_normal((m, k)).astype(np.float32), rng.standard_normal((k, n)).astype(np.float32)
+    x[:, 3] = np.ldexp(x[:, 3], -50)
+    w[4] = np.ldexp(w[4], -20)
+    x[1::2, :k // 2] = 0
+    x[::2, k // 2:] = 0
+    w[:k // 2, 1::2] = 0
+    w[k // 2:, ::2] = 0
+    y, _ = bo.run_linear(hip, x, w, None, None, "none", F32)
+    assert not y[::2, 1::2].any() and not y[1::2, ::2].any()
+    rows, cols = _some(m), _some(n)
+    want, mag = _reference(x, w.T, rows, cols)
+    within(y[rows][:, cols], want, _sum_bound(k, mag, want))
+
+
+@pytest.mark.parametrize("shape,kernel", [((2100, 300, 1900), "thvm_gemm_64x64_f32"), ((2000, 1801, 1900), "thvm_gemm_128x128_f32")], ids=str)
+@pytest.mark.parametrize("far", [10, 25, 60])
+def test_one_large_feature(hip, shape, kernel, far):
+    """One input and one output far above the others, which then are faint
+    in every row and column; every second output does not see the large one."""
+    m, k, n = shape
+    assert bp.linear(m, k, n, F32)[-1] == kernel
+    rng = np.random.default_rng(far)
+    x, w = rng.standard_normal((m, k)).astype(np.float32), rng.standard_normal((k, n)).astype(np.float32)
+    x[:, 5] = np.ldexp(x[:, 5], far)
+    w[:, 6] = np.ldexp(w[:, 6], far)
+    w[5, ::2] = 0
+    y, _ = bo.run_linear(hip, x, w, None, None, "none", F32)
+    rows, cols = _some(m), _some(n, 80)
+    want, mag = _reference(x, w.T, rows, cols)
+    within(y[rows][:, cols], want, _sum_bound(k, mag, want))

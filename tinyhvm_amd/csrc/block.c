@@ -294,7 +294,7 @@ static int lies_well(u32 cols, u32 dtype) { return dtype == DTYPE_F16 && cols % 
 
 static void packed_carve(Packed *p, Carve *c, u32 dtype) {
     p->p = carve(c, packed_bytes(p, dtype) + PACK_SLACK);
-    p->e = carve(c, dtype == DTYPE_F32 ? p->Rp * 4ull : 0);
+    p->e = carve(c, dtype == DTYPE_F32 ? p->Rp * 8ull : 0);
 }
 
 /* A product's tile and K splits: C [M][N] over K. */
@@ -404,9 +404,6 @@ static int pack(const Source *src, u32 n, u32 dtype) {
         a.row_part = m->rows ? m->row_part : 0;
         a.col_part = m->cols ? m->col_part : 0;
         a.sum_part = m->sums ? m->sum_part : 0;
-        z.first[i] = (u32)sized;
-        z.p[i] = a;
-        sized += (u64)m->row_parts * m->col_parts;
         u32 rmax = m->rows || m->cols || dtype == DTYPE_F16 ? (u32)round_up(m->R ? m->R : 1, 64) : 64, cmax = (u32)round_up(m->C ? m->C : 1, 64);
         if (m->rows) {
             a.pn = m->rows->p; a.en = m->rows->e; a.Rn = m->rows->Rp; a.KBn = m->rows->KB;
@@ -420,8 +417,11 @@ static int pack(const Source *src, u32 n, u32 dtype) {
         if (m->sums) sums = i + 1;
         a.ctiles = cmax / 64;
         s.first[i] = (u32)tiles;
-        s.p[i] = a;
+        z.first[i] = (u32)sized;
+        s.p[i] = z.p[i] = a;
         tiles += (u64)(rmax / 64) * a.ctiles;
+        /* of a matrix of nothing a workgroup clears the rows' numbers */
+        sized += m->row_parts && m->col_parts ? (u64)m->row_parts * m->col_parts : 1;
     }
     s.n = z.n = n;
     int rc = THVM_HIP_OK;

@@ -38,7 +38,7 @@ typedef struct {
 /* C[M][N] = sum over k of A[r][k] B[c][k], packed operands (gemm_kernels.hip) */
 typedef struct {
     u64 A, B;                  /* packed; KB blocks of 16 k */
-    u64 ea, eb;                /* exponents of A's and B's rows (32-bit operands) */
+    u64 ea, eb;                /* of each row of A and of B its exponent and number of faint values (32-bit operands) */
     Origin oa, ob;             /* what the packed operands were */
     u64 out, z, bias, res;     /* row-major [M][N]; bias [N] */
     u64 part, count;           /* the K splits' sums, and how many of a tile's are there (0 between launches) */
@@ -54,7 +54,7 @@ typedef struct {
 typedef struct {
     u64 src, z;                /* z 0: the matrix itself */
     u64 pn, pt;                /* packed with rows r (Rn of them, KBn blocks of k = c); with rows c */
-    u64 en, et;                /* their exponents */
+    u64 en, et;                /* of each of their rows its exponent and number of faint values */
     u64 row_part, col_part;    /* the largest magnitudes' bits [row_parts][R], [col_parts][C] */
     u64 sum_part;              /* column sums [..][C] f32 */
     u64 stride;                /* bytes between the matrices of a batch in pn and pt */

@@ -19,14 +19,17 @@
 // 32-bit operands are two f16 planes: x 2^e = hi + lo, hi the nearest f16 and
 // lo the nearest f16 of what is left, with e such that the largest value of
 // the row (the products' sums never mix rows) lies in [2^14, 2^15). hi + lo
-// is x 2^e to 2^-24 of itself, or to 2^-25 where x is under 2^-15 of its
-// row's largest. Of the four products three are summed, hi hi + hi lo +
-// lo hi; lo lo is at most 2^-24 of the product. All sums are 32 bits. So a
-// 32-bit product costs three 16-bit ones, where three bf16 planes cost six.
-// A sum that is not finite, as each is that an infinity or NaN goes into, is
-// computed again from the operands as the caller has them, in 32-bit sums of
-// 32-bit products (block_again): of 4096^3 with a NaN in every row 2.0 ms, in one
-// row 0.72, in none 0.42.
+// is x 2^e to 2^-23 of itself, or to 2^-25 where x 2^e is under 2^-2. Of the
+// four products three are summed, hi hi + hi lo + lo hi; lo lo is at most 2^-22
+// of the product. All sums are 32 bits. So a 32-bit product costs three 16-bit
+// ones, where three bf16 planes cost six, and a sum is within (2 K + 8) 2^-24
+// of its products' magnitudes (a 32-bit one: K 2^-24), with two exceptions:
+//   a sum that is not finite, as each is that an infinity or NaN goes into;
+//   a sum of products that are all small beside their row's and column's
+//   largest, of rows with values that lost bits (doubtful).
+// Those are computed again from the operands as the caller has them, in 32-bit
+// sums of 32-bit products (block_again): of 4096^3 with a NaN in every row 2.0
+// ms, in one row 0.72, in none 0.42.
 // 16-bit operands are one plane as they are.
 //
 // Large tiles: of 4096^3 in 16 bits as they lie 135 us, 1018 TFLOP/s (a library
@@ -123,6 +126,19 @@ __device__ __forceinline__ void split(float v, f16 &hi, f16 &lo) {
     hi = (f16)v;
     const float h = (float)hi;
     lo = fabsf(h) < __builtin_inff() ? (f16)(v - h) : (f16)0.0f;
+}
+
+// Of packed 32-bit operands each row has its exponent (ROW_EMPTY where all
+// values are 0), and the number of its faint values: under 2^-2 as they are
+// packed, and not 0, so that lo may have lost bits, 2^-24 at most. Partners are
+// under 2^15, so faint values move a sum by (their number in both rows) 2^-9
+// at most: by less than K 2^-25 of the sum of the products' magnitudes, if that
+// is over the number times 2^16 / K.
+#define ROW_EMPTY 0x4000
+typedef int Row __attribute__((ext_vector_type(2)));      // exponent, faint values
+__device__ __forceinline__ float faint_unit(u32 K) { return 65536.0f * __builtin_amdgcn_rcpf((float)K); }
+__device__ __forceinline__ bool doubtful(Row r, Row c, float unit, float v) {
+    return r.x != ROW_EMPTY && c.x != ROW_EMPTY && fabsf(v) < (float)((u32)r.y + (u32)c.y) * unit;
 }
 
 // ---- the product ----
@@ -409,6 +425,56 @@ __device__ __forceinline__ f16v block_again(const GemmArgs &a, u32 rb, u32 cb) {
     return acc;
 }
 
+// A wave's staged strip of 32 rows: small sums of faint values stand where the
+// products' magnitudes (up to as many as it takes to say so) add up to enough,
+// or where no product is other than 0; the others become NaN, to be computed
+// again. A value's magnitude is that of hi, and lo's where hi is 0, which are
+// not both 0 (count_faint).
+template <typename TL>
+__device__ __forceinline__ void weigh_doubtful(const GemmArgs &a, float *st, u32 rb, u32 cb) {
+    const u32 lane = threadIdx.x & 63u, h = (lane >> 5) * 4;
+    const float unit = faint_unit(a.K);
+    typedef unsigned short us8 __attribute__((ext_vector_type(8)));
+    auto magnitude = [](const glob<f16> *p) {
+        const us8 hi = *(const glob<us8> *)p & (unsigned short)0x7FFF, lo = *(const glob<us8> *)(p + 512) & (unsigned short)0x7FFF;
+        return __builtin_bit_cast(h8, __builtin_elementwise_max(hi, lo));
+    };
+#pragma unroll 1
+    for (u32 j = 0; j < TL::NI; j++, cb += 32) {
+        const glob<Row> *row = (const glob<Row> *)a.ea + rb + h;
+        const Row col = ((const glob<Row> *)a.eb)[cb + (lane & 31u)];
+        float *at = st + h * TL::PITCH + j * 32 + (lane & 31u);
+        u32 open = 0, most = 0;
+#pragma unroll
+        for (u32 t = 0; t < 16; t++) {
+            const u32 r = (t >> 2) * 8 + (t & 3u);
+            const Row w = row[r];
+            open |= doubtful(w, col, unit, at[r * TL::PITCH]) ? 1u << t : 0u;
+            most = max(most, (u32)w.y + (u32)col.y);
+        }
+        const float enough = (float)most * unit;
+        const glob<f16> *A = (const glob<f16> *)a.A + block_at<TL::PL>(rb >> 5, 0, a.KB, 0) + lane * 8u;
+        const glob<f16> *B = (const glob<f16> *)a.B + block_at<TL::PL>(cb >> 5, 0, a.KB, 0) + lane * 8u;
+        f16v sum = 0.0f;
+#pragma unroll 1
+        for (u32 kb = 0; kb < a.KB && __ballot(open != 0); kb += 2) {
+            h8 x[2], w[2];
+#pragma unroll
+            for (u32 q = 0; q < 2; q++) x[q] = magnitude(A + q * (TL::PL * 512u)), w[q] = magnitude(B + q * (TL::PL * 512u));
+#pragma unroll
+            for (u32 q = 0; q < 2; q++) sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[q], w[q], sum, 0, 0, 0);
+            A += TL::PL * 1024u, B += TL::PL * 1024u;
+#pragma unroll
+            for (u32 t = 0; t < 16; t++) open &= sum[t] >= enough ? ~(1u << t) : ~0u;
+        }
+#pragma unroll
+        for (u32 t = 0; t < 16; t++)
+            if (((open >> t) & 1u) && sum[t] > 0.0f) at[((t >> 2) * 8 + (t & 3u)) * TL::PITCH] = __builtin_nanf("");
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // What an output becomes: z = sum (+ bias), y = act(z) (+ residual).
 template <typename T>
 __device__ __forceinline__ void finish1(const GemmArgs &a, u32 r, u32 c, float v) {
@@ -537,11 +603,19 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs &a, f16 *lds) {
     const bool whole = c + 8 <= a.N;
     float bias[8];
     int ec[8];
+    u32 nc = 0;            // the columns' most faint values
+    const float unit = faint_unit(a.K);
     u32 later[TL::MI];      // outputs of row block i that are not finished yet: bit 8 p + j
     if (a.bias) load8<T>((const glob<T> *)a.bias, c, a.N, bias);
     if (TL::PL == 2)
 #pragma unroll
-        for (u32 j = 0; j < 8; j++) ec[j] = ((const glob<int> *)a.eb)[c + j];
+        for (u32 j = 0; j < 8; j++) {
+            const Row w = ((const glob<Row> *)a.eb)[c + j];
+            ec[j] = w.x;
+            nc = max(nc, (u32)w.y);
+        }
+    // (with both, the largest 32-bit tile would not fit the registers)
+    constexpr bool AHEAD = TL::PL == 1 || TL::MI < 4;
     any_vec<T, 8> res[2][PASSES];
     auto ask = [&](u32 i, any_vec<T, 8> (&x)[PASSES]) {
 #pragma unroll
@@ -553,9 +627,15 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs &a, f16 *lds) {
     ask(0, res[0]);
 #pragma unroll
     for (u32 i = 0; i < TL::MI; i++) {
-        if (i + 1 < TL::MI) ask(i + 1, res[(i + 1) & 1]);
+        if (AHEAD && i + 1 < TL::MI) ask(i + 1, res[(i + 1) & 1]);
+        if (!AHEAD && i) ask(i, res[i & 1]);
+        Row rows[PASSES];
+        if (TL::PL == 2 && AHEAD)
+#pragma unroll
+            for (u32 p = 0; p < PASSES; p++) rows[p] = ((const glob<Row> *)a.ea)[r0 + i * 32 + p * RPP];      // there are whole tiles of them
         stage_rows<TL>(st, acc[i]);
         later[i] = 0;
+        u32 odd = 0;       // groups of 8 columns that may hold such
 #pragma unroll
         for (u32 p = 0; p < PASSES; p++) {
             const u32 r = r0 + i * 32 + p * RPP;
@@ -564,22 +644,21 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs &a, f16 *lds) {
             *(f4 *)v = *(const f4 *)(row + p * RPP * TL::PITCH);
             *(f4 *)(v + 4) = *(const f4 *)(row + p * RPP * TL::PITCH + 4);
             if (TL::PL == 2) {
+                if (!AHEAD) rows[p] = ((const glob<Row> *)a.ea)[r];
                 u32 most = 0;
+                float least = __builtin_inff();
 #pragma unroll
-                for (u32 j = 0; j < 8; j++) most = max(most, __float_as_uint(v[j]) & 0x7FFFFFFFu);
-                const int er = ((const glob<int> *)a.ea)[r];
-                if (most >= 0x7F800000u) {
-                    // one by one, those that stand
-#pragma unroll 1
-                    for (u32 j = 0; j < 8 && c + j < a.N; j++) {
-                        const float x = row[p * RPP * TL::PITCH + j];
-                        if (fabsf(x) < __builtin_inff()) finish1<T>(a, r, c + j, ldexpf(x, -(er + ((const glob<int> *)a.eb)[c + j])));
-                        else later[i] |= 1u << (p * 8 + j);
-                    }
+                for (u32 j = 0; j < 8; j++) most = max(most, __float_as_uint(v[j]) & 0x7FFFFFFFu), least = fminf(least, fabsf(v[j]));
+                bool some = most >= 0x7F800000u;
+                if (least < (float)((u32)rows[p].y + nc) * unit)
+#pragma unroll
+                    for (u32 j = 0; j < 8; j++) some |= doubtful(rows[p], Row{ec[j], (int)nc}, unit, v[j]);
+                if (some) {
+                    odd |= 1u << p;
                     continue;
                 }
 #pragma unroll
-                for (u32 j = 0; j < 8; j++) v[j] = ldexpf(v[j], -(er + ec[j]));
+                for (u32 j = 0; j < 8; j++) v[j] = ldexpf(v[j], -(rows[p].x + ec[j]));
             }
             if (a.bias)
 #pragma unroll
@@ -597,6 +676,18 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs &a, f16 *lds) {
                         if (c + j < a.N) v[j] += (float)((const glob<T> *)a.res)[at + c + j];
             }
             store8<T>((glob<T> *)a.out + at, c, a.N, v);
+        }
+        if (TL::PL == 2 && __ballot(odd != 0)) {
+            weigh_doubtful<TL>(a, st, ti * TL::TM + ((wave / TL::WN) * TL::MI + i) * 32, tj * TL::TN + (wave % TL::WN) * TL::NI * 32);
+#pragma unroll 1
+            for (u32 b = 0; b < PASSES * 8; b++) {
+                if (!((odd >> b / 8) & 1u) || c + b % 8 >= a.N) continue;
+                const u32 r = r0 + i * 32 + b / 8 * RPP;
+                const float x = row[b / 8 * RPP * TL::PITCH + b % 8];
+                if (fabsf(x) < __builtin_inff())
+                    finish1<T>(a, r, c + b % 8, ldexpf(x, -(((const glob<Row> *)a.ea)[r].x + ((const glob<Row> *)a.eb)[c + b % 8].x)));
+                else later[i] |= 1u << b;
+            }
         }
     }
     if (TL::PL == 2)
@@ -867,6 +958,10 @@ template <typename T>
 __device__ __forceinline__ void pack_sizes(const PackArgs &a, u32 block) {
     __shared__ u32 lw[8][512];
     __shared__ float ls[8][512];
+    const u32 threads = max(a.row_parts * a.col_parts, 1u) * 512u;
+    for (u32 i = block * 512u + threadIdx.x; i < a.Rn; i += threads) ((glob<u32> *)a.en)[2u * i + 1u] = 0;
+    for (u32 i = block * 512u + threadIdx.x; i < a.Ct; i += threads) ((glob<u32> *)a.et)[2u * i + 1u] = 0;
+    if (!a.R || !a.C) return;
     const u32 bx = block % a.row_parts, by = block / a.row_parts;
     pack_sizes_of<T>(a, bx, by, lw, ls);
     __syncthreads();
@@ -878,6 +973,26 @@ __device__ __forceinline__ void pack_sizes(const PackArgs &a, u32 block) {
     for (u32 k = 1; k < 8; k++) w = max(w, lw[k][t]), s += ls[k][t];
     if (a.col_part) ((glob<u32> *)a.col_part)[(u64)by * a.C + ct] = w;
     if (a.sum_part) ((glob<float> *)a.sum_part)[(u64)by * a.C + ct] = s;
+}
+
+// The faint ones of 8 values of row r, for its count (pack_sizes has cleared
+// it). Those that the planes would not hold
+// at all become the least that they hold. Shifted left, magnitudes lose their
+// sign and compare as before, and 0 less 1 is the largest of all.
+__device__ __forceinline__ void count_faint(u64 words, u32 r, float *v) {
+    constexpr u32 faint = (0x3E800000u << 1) - 1u;      // 2^-2
+    u32 least = ~0u;
+#pragma unroll
+    for (u32 j = 0; j < 8; j++) least = min(least, (__float_as_uint(v[j]) << 1) - 1u);
+    if (least >= faint) return;
+    u32 n = 0;
+#pragma unroll
+    for (u32 j = 0; j < 8; j++)
+        if ((__float_as_uint(v[j]) << 1) - 1u < faint) {
+            n++;
+            v[j] = copysignf(fmaxf(fabsf(v[j]), 5.9604645e-8f), v[j]);      // 2^-24
+        }
+    __hip_atomic_fetch_add((u32 *)words + 2u * r + 1u, n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 // A 64 x 64 tile of a matrix [R][C] into one or both packed orientations:
@@ -906,8 +1021,8 @@ __device__ __forceinline__ void pack_tile(const PackArgs &a, const MuonArgs *mu,
         if (q == 0) {
             er[i] = exp_of(wr);
             ec[i] = exp_of(wc);
-            if (a.pn && c0 == 0 && r0 + i < a.Rn) ((glob<int> *)a.en)[r0 + i] = er[i];
-            if (a.pt && r0 == 0 && c0 + i < a.Ct) ((glob<int> *)a.et)[c0 + i] = ec[i];
+            if (a.pn && c0 == 0 && r0 + i < a.Rn) ((glob<int> *)a.en)[2u * (r0 + i)] = wr ? er[i] : ROW_EMPTY;
+            if (a.pt && r0 == 0 && c0 + i < a.Ct) ((glob<int> *)a.et)[2u * (c0 + i)] = wc ? ec[i] : ROW_EMPTY;
         }
     }
     if (PL == 2 && !MUON && a.sum_out && r0 == 0 && t < 64 && c0 + t < a.C) {
@@ -954,6 +1069,7 @@ __device__ __forceinline__ void pack_tile(const PackArgs &a, const MuonArgs *mu,
             if (PL == 2 && !MUON)
 #pragma unroll
                 for (u32 k = 0; k < 8; k++) v[k] = ldexpf(v[k], er[i]);
+            if (PL == 2 && !MUON) count_faint(a.en, r, v);
             put_packed<PL>(pn, a.KBn, r, c, v);
         }
     }
@@ -969,6 +1085,7 @@ __device__ __forceinline__ void pack_tile(const PackArgs &a, const MuonArgs *mu,
                 v[k] = tile[i + k][j];
                 if (PL == 2 && !MUON) v[k] = ldexpf(v[k], ec[j]);
             }
+            if (PL == 2 && !MUON) count_faint(a.et, c, v);
             put_packed<PL>(pt, a.KBt, c, r, v);
         }
     if (PL == 1 && a.sum_part && t < 64 && c0 + t < a.C && r0 < a.R) {
