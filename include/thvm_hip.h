@@ -187,7 +187,8 @@ int  thvm_hip_linear(u32 y, u32 z, u32 x, u32 w, u32 bias, u32 res, u32 act, u32
 /* Its gradient from dy and the kept z (not read without an activation): with
  * dz = dy act'(z), dx = dz W^T, dw = x^T dz, db = the column sums of dz. That
  * of res is dy itself. Any of the three may be absent, x without dw and w
- * without dx. Of DTYPE_F16, the products take dz rounded to 16 bits. */
+ * without dx. Of DTYPE_F16, the products take dz rounded to 16 bits, or as it
+ * is where that would be an infinity. */
 int  thvm_hip_linear_grad(u32 dx, u32 dw, u32 db, u32 dy, u32 z, u32 x, u32 w, u32 act, u32 m, u32 k, u32 n, u32 dtype);
 /* One step of an optimiser whose update is orthogonalised, on `count`
  * matrices [rows][cols] of one shape, each with its gradient and its momentum

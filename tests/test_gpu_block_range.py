@@ -9,7 +9,7 @@ import pytest
 
 from tests import blockops as bo
 from tests import blockplan as bp
-from tests.blockops import F32, U32
+from tests.blockops import F16, F32, U32
 from tests.test_gpu_block import within
 
 pytestmark = pytest.mark.gpu
@@ -204,3 +204,40 @@ def test_one_large_feature(hip, shape, kernel, far):
     rows, cols = _some(m), _some(n, 80)
     want, mag = _reference(x, w.T, rows, cols)
     within(y[rows][:, cols], want, _sum_bound(k, mag, want))
+
+
+# ---- 16-bit gradients whose dy act'(z) is out of 16 bits ----
+
+@pytest.mark.parametrize("shape", [(70, 90, 110), (1500, 1601, 1499)], ids=str)
+def test_16_bit_gradient_past_the_range(hip, shape):
+    """dy under 65504 and a slope of 1.13: the gradients are those of the
+    product, which 32 bits hold, and not infinities."""
+    m, k, n = shape
+    rng = np.random.default_rng(m)
+    x, w = (rng.standard_normal((m, k)) / 256).astype(np.float16), (rng.standard_normal((k, n)) / 256).astype(np.float16)
+    dy, z = rng.standard_normal((2, m, n)).astype(np.float16)
+    dy[3, 5], z[3, 5] = 60000, 1.4
+    dy[m - 1, n - 1], z[m - 1, n - 1] = -65504, 1.5
+    w[::2, 5] = 0
+    x[3, 1::2] = 0
+    s = bo.slope("gelu", z)
+    dz = dy.astype(np.float64) * s
+    assert np.abs(dz).max() > 65520
+    dx, dw, db = bo.run_linear_grad(hip, dy, z, x, w, "gelu", F16)
+    # act' in 32 bits; dz is rounded to 16 bits
+    edz = np.abs(dy.astype(np.float64)) * (16 * U32 * (1 + np.abs(z.astype(np.float64)))) + np.abs(dz) * 2.0 ** -11 + 2.0 ** -25
+    rows, cols = np.union1d(_some(m), [3]), _some(k)
+    w64, x64 = w.astype(np.float64), x.astype(np.float64)
+    want = dz[rows] @ w64[cols].T
+    mag = np.abs(dz[rows]) @ np.abs(w64[cols]).T
+    within(dx[rows][:, cols], want, (n + 4) * U32 * mag + edz[rows] @ np.abs(w64[cols]).T + bo.rounding(F16, want))
+    rows, cols = _some(k), np.union1d(_some(n), [5])
+    want = x64[:, rows].T @ dz[:, cols]
+    mag = np.abs(x64[:, rows]).T @ np.abs(dz[:, cols])
+    within(dw[rows][:, cols], want, (m + 4) * U32 * mag + np.abs(x64[:, rows]).T @ edz[:, cols] + bo.rounding(F16, want))
+    # the column that holds the value is within 16 bits again once rounded, or an infinity
+    want = dz.sum(0)
+    fits = np.abs(want) < 65500
+    bound = (edz - np.abs(dz) * 2.0 ** -11).sum(0) + (m + 4) * U32 * np.abs(dz).sum(0) + bo.rounding(F16, want)
+    within(db[fits], want[fits], bound[fits])
+    assert np.isinf(db[~fits]).sum() == (np.abs(want[~fits]) > 65520).sum()

@@ -21,7 +21,8 @@ extern const unsigned char thvm_norm_kernels_co[], thvm_gemm_kernels_co[];
 static struct {
     hipModule_t mod[MODULES];
     struct { char name[48]; hipFunction_t fn; } fn[KERNELS];
-    u64 counts, counts_cap;     /* [COUNTS] u32: 0 between launches */
+    u64 counts, counts_cap;     /* [COUNTS] u32: 0 between launches; and one more, see past16 */
+    u32 call;                   /* of a gradient */
 } B;
 static Scratch block_ws;
 
@@ -44,8 +45,8 @@ int block_init(void) {
             return -1;
         }
     }
-    u32 n = COUNTS, zero = 0;
-    void *counts = pool_block_get(4ull * COUNTS, &B.counts_cap);
+    u32 n = COUNTS + 1, zero = 0;
+    void *counts = pool_block_get(4ull * n, &B.counts_cap);
     hipFunction_t fill = rtc_static_fn("thvm_fill_u32");
     if (!counts || !fill) return -1;
     B.counts = (u64)(uintptr_t)counts;
@@ -373,6 +374,11 @@ typedef struct {
     u32 rt, row_parts, col_parts;
 } Source;
 
+/* Whether a 16-bit dz of a call is past its type's range: packing writes the
+ * call's number here, so that there is nothing to clear between calls (a
+ * graph's launches share theirs: one that had such a dz has the next look, too). */
+static u64 past16(void) { return B.counts + 4ull * COUNTS; }
+
 #define SIZE_COLS 512u
 #define SIZE_PARTS 64u
 static void source_carve(Source *s, Carve *c, u32 dtype) {
@@ -414,6 +420,7 @@ static int pack(const Source *src, u32 n, u32 dtype) {
             if (a.Ct > cmax) cmax = a.Ct;
         }
         a.sum_out = m->sums;
+        a.past16 = past16(); a.call = B.call;
         if (m->sums) sums = i + 1;
         a.ctiles = cmax / 64;
         s.first[i] = (u32)tiles;
@@ -644,6 +651,8 @@ int thvm_hip_linear_grad(u32 dx, u32 dw, u32 db, u32 dy, u32 z, u32 x, u32 w, u3
     operands_ready(o, 7);
     GemmArgs a;
     memset(&a, 0, sizeof a);
+    if (!++B.call) B.call = 1;
+    a.past16 = act ? past16() : 0; a.call = B.call;
     int rc = pack(src, ns, dtype);
     if (dx && !rc) {
         a.out = addr(dx);

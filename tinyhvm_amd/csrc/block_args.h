@@ -40,11 +40,13 @@ typedef struct {
     u64 A, B;                  /* packed; KB blocks of 16 k */
     u64 ea, eb;                /* of each row of A and of B its exponent and number of faint values (32-bit operands) */
     Origin oa, ob;             /* what the packed operands were */
+    u64 past16;                /* holds `call` if a 16-bit dz is past its type's range */
     u64 out, z, bias, res;     /* row-major [M][N]; bias [N] */
     u64 part, count;           /* the K splits' sums, and how many of a tile's are there (0 between launches) */
     u32 M, N, KB, tm, tn, splits, act;
     u32 K, lda, ldb;           /* operands as they lie */
     u32 kper;                  /* few rows: A is x [M][K], B is W [K][N], kper k a split */
+    u32 call;
 } GemmArgs;
 
 /* few rows: the longest K split of a workgroup, whose part of x it holds in LDS */
@@ -61,7 +63,8 @@ typedef struct {
     u32 R, C, act, rt;         /* rt: rows of a column part */
     u32 Rn, KBn, Ct, KBt, row_parts, col_parts;
     u64 sum_out;               /* [C]: the column sums (32-bit operands) */
-    u32 ctiles, pad;           /* tiles of 64 columns */
+    u64 past16;                /* as in GemmArgs */
+    u32 ctiles, call;          /* tiles of 64 columns */
 } PackArgs;
 
 /* up to three matrices of one launch: p[i] from workgroup first[i] on */

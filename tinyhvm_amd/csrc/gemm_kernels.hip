@@ -30,7 +30,12 @@
 // Those are computed again from the operands as the caller has them, in 32-bit
 // sums of 32-bit products (block_again): of 4096^3 with a NaN in every row 2.0
 // ms, in one row 0.72, in none 0.42.
-// 16-bit operands are one plane as they are.
+// 16-bit operands are one plane as they are, and so is a gradient's dz = dy
+// act'(z), rounded to 16 bits as a network in 16 bits holds it: of 2048^3 its
+// products' error against 64 bits is 2.9e-4, that of dz in 32 bits 2.1e-4, most
+// of it the outputs' own rounding, and a second plane for dz would double the
+// products' time. Where a dz is past 16 bits, the sums that it goes into are
+// computed again, too; packing tells the products of a call that there is one.
 //
 // Large tiles: of 4096^3 in 16 bits as they lie 135 us, 1018 TFLOP/s (a library
 // product 1155 on the same card; packed ones alone 129 us), the matrix units
@@ -475,6 +480,11 @@ __device__ __forceinline__ void weigh_doubtful(const GemmArgs &a, float *st, u32
     __builtin_amdgcn_wave_barrier();
 }
 
+// Whether 8 sums are finite (or not, if they add up to over 2^128).
+__device__ __forceinline__ bool all_finite(const float *v) {
+    return fabsf(((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]))) < __builtin_inff();
+}
+
 // What an output becomes: z = sum (+ bias), y = act(z) (+ residual).
 template <typename T>
 __device__ __forceinline__ void finish1(const GemmArgs &a, u32 r, u32 c, float v) {
@@ -587,6 +597,9 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs &a, f16 *lds) {
     tile_of(blockIdx.x, a.tm, a.tn, ti, tj);
     const u32 S = a.KB / TL::US, per = (S / TL::TURN + a.splits - 1) / a.splits * TL::TURN, s0 = blockIdx.y * per;
     const u32 s1 = s0 + per < S ? s0 + per : S;
+    // a gradient whose 16-bit dz are infinities where dy act'(z) is not (asked for early)
+    constexpr bool PACKED16 = TL::PL == 1 && MA == PACKED;
+    const u32 past = PACKED16 && a.past16 ? *(const glob<u32> *)a.past16 : 0u;
     f16v acc[TL::MI][TL::NI];
     const Operand A = operand<TL, MA>(a.A, a.lda, a.M, ti * TL::TM, a.KB, a.K, s0);
     const Operand B = operand<TL, MB>(a.B, a.ldb, a.N, tj * TL::TN, a.KB, a.K, s0);
@@ -635,31 +648,56 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs &a, f16 *lds) {
             for (u32 p = 0; p < PASSES; p++) rows[p] = ((const glob<Row> *)a.ea)[r0 + i * 32 + p * RPP];      // there are whole tiles of them
         stage_rows<TL>(st, acc[i]);
         later[i] = 0;
-        u32 odd = 0;       // groups of 8 columns that may hold such
+        // groups of 8 columns with sums that are computed again (not finite ones
+        // by now): known for all rows ahead of the rest, which has no branches for it
+        u32 odd = 0;
+        float all[PASSES][8];
+        auto read = [&]() {
+#pragma unroll
+            for (u32 p = 0; p < PASSES; p++) {
+                *(f4 *)all[p] = *(const f4 *)(row + p * RPP * TL::PITCH);
+                *(f4 *)(all[p] + 4) = *(const f4 *)(row + p * RPP * TL::PITCH + 4);
+            }
+        };
+        auto look = [&]() {
+            odd = 0;
+#pragma unroll
+            for (u32 p = 0; p < PASSES; p++) odd |= !all_finite(all[p]) ? 1u << p : 0u;
+        };
+        read();
+        if (TL::PL == 2) {
+            bool small = false, doubt = false;
+#pragma unroll
+            for (u32 p = 0; p < PASSES; p++) {
+                if (!AHEAD) rows[p] = ((const glob<Row> *)a.ea)[r0 + i * 32 + p * RPP];
+                float least = fabsf(all[p][0]);
+#pragma unroll
+                for (u32 j = 1; j < 8; j++) least = fminf(least, fabsf(all[p][j]));
+                small |= least < (float)((u32)rows[p].y + nc) * unit;
+            }
+            look();
+            if (__builtin_expect(__ballot(small) != 0, 0)) {
+#pragma unroll
+                for (u32 j = 0; j < 8; j++) {
+                    const Row w = ((const glob<Row> *)a.eb)[c + j];
+#pragma unroll
+                    for (u32 p = 0; p < PASSES; p++) doubt |= doubtful(rows[p], w, unit, all[p][j]);
+                }
+                if (__ballot(doubt)) {
+                    weigh_doubtful<TL>(a, st, ti * TL::TM + ((wave / TL::WN) * TL::MI + i) * 32, tj * TL::TN + (wave % TL::WN) * TL::NI * 32);
+                    read();
+                    look();
+                }
+            }
+        } else if (PACKED16 && __builtin_expect(past && past == a.call, 0)) look();
 #pragma unroll
         for (u32 p = 0; p < PASSES; p++) {
             const u32 r = r0 + i * 32 + p * RPP;
-            if (r >= a.M || c >= a.N) continue;
-            float v[8];
-            *(f4 *)v = *(const f4 *)(row + p * RPP * TL::PITCH);
-            *(f4 *)(v + 4) = *(const f4 *)(row + p * RPP * TL::PITCH + 4);
-            if (TL::PL == 2) {
-                if (!AHEAD) rows[p] = ((const glob<Row> *)a.ea)[r];
-                u32 most = 0;
-                float least = __builtin_inff();
-#pragma unroll
-                for (u32 j = 0; j < 8; j++) most = max(most, __float_as_uint(v[j]) & 0x7FFFFFFFu), least = fminf(least, fabsf(v[j]));
-                bool some = most >= 0x7F800000u;
-                if (least < (float)((u32)rows[p].y + nc) * unit)
-#pragma unroll
-                    for (u32 j = 0; j < 8; j++) some |= doubtful(rows[p], Row{ec[j], (int)nc}, unit, v[j]);
-                if (some) {
-                    odd |= 1u << p;
-                    continue;
-                }
+            if (r >= a.M || c >= a.N || ((odd >> p) & 1u)) continue;
+            float (&v)[8] = all[p];
+            if (TL::PL == 2)
 #pragma unroll
                 for (u32 j = 0; j < 8; j++) v[j] = ldexpf(v[j], -(rows[p].x + ec[j]));
-            }
             if (a.bias)
 #pragma unroll
                 for (u32 j = 0; j < 8; j++) v[j] += bias[j];
@@ -677,20 +715,22 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs &a, f16 *lds) {
             }
             store8<T>((glob<T> *)a.out + at, c, a.N, v);
         }
-        if (TL::PL == 2 && __ballot(odd != 0)) {
-            weigh_doubtful<TL>(a, st, ti * TL::TM + ((wave / TL::WN) * TL::MI + i) * 32, tj * TL::TN + (wave % TL::WN) * TL::NI * 32);
+        if ((TL::PL == 2 || PACKED16) && __builtin_expect(__ballot(odd != 0) != 0, 0))
+            // one by one, those that stand
 #pragma unroll 1
             for (u32 b = 0; b < PASSES * 8; b++) {
-                if (!((odd >> b / 8) & 1u) || c + b % 8 >= a.N) continue;
                 const u32 r = r0 + i * 32 + b / 8 * RPP;
+                if (!((odd >> b / 8) & 1u) || r >= a.M || c + b % 8 >= a.N) continue;
                 const float x = row[b / 8 * RPP * TL::PITCH + b % 8];
                 if (fabsf(x) < __builtin_inff())
-                    finish1<T>(a, r, c + b % 8, ldexpf(x, -(((const glob<Row> *)a.ea)[r].x + ((const glob<Row> *)a.eb)[c + b % 8].x)));
+                    finish1<T>(a, r, c + b % 8, TL::PL == 1 ? x : ldexpf(x, -(((const glob<Row> *)a.ea)[r].x + ((const glob<Row> *)a.eb)[c + b % 8].x)));
                 else later[i] |= 1u << b;
             }
-        }
     }
-    if (TL::PL == 2)
+    u32 any = 0;
+#pragma unroll
+    for (u32 i = 0; i < TL::MI; i++) any |= later[i];
+    if ((TL::PL == 2 || PACKED16) && __builtin_expect(__ballot(any != 0) != 0, 0))
 #pragma unroll 1
         for (u32 i = 0; i < TL::MI; i++) {
             u32 mine = later[0];
@@ -1061,6 +1101,12 @@ __device__ __forceinline__ void pack_tile(const PackArgs &a, const MuonArgs *mu,
 #pragma unroll
                 for (u32 k = 0; k < 8; k++) v[k] *= unit_lds;
             } else source<T, 8>(a, r, c, v);
+        }
+        if (PL == 1 && !MUON && a.z) {
+            float most = 0.0f;
+#pragma unroll
+            for (u32 k = 0; k < 8; k++) most = fmaxf(most, fabsf(v[k]));
+            if (most >= 65520.0f) *(glob<u32> *)a.past16 = a.call;
         }
         if (a.pt || a.sum_part)
 #pragma unroll
