@@ -164,6 +164,9 @@ int  thvm_hip_dispatch_uop_kernel_noalloc(u32 out_buf, const u32 *leaf_bufs, u32
 #define THVM_HIP_ACT_GELU 2       /* z (1 + erf(z / sqrt 2)) / 2 */
 #define THVM_HIP_ACT_GELU_TANH 3  /* its tanh form */
 #define THVM_HIP_ACT_SILU 4       /* z / (1 + exp -z) */
+/* An activation of a 32-bit z is within 8 + b units of 2^-24 of itself (or within
+ * 2^-120), b = 2 z^2 for gelu, 10 (|z| + 0.045 |z|^3) for its tanh form, 2 |z| for
+ * silu and 0 else; its slope act' within 16 (1 + |z|) 2^-24. */
 /* Layer norm of the rows of x [rows][cols]: y = (x - mean) * rstd * gamma +
  * beta, rstd = 1 / sqrt(variance + eps). gamma and beta [cols] may be absent
  * (1 and 0); mean and rstd [rows] f32 are kept where given, NaN of rows of no

@@ -95,3 +95,52 @@ def test_infinities_through_an_activation(hip, dt, name):
     assert np.all(y[:, 0] == np.inf) and np.isfinite(y[:, 2:]).all()
     low = {"none": -np.inf, "relu": 0.0}.get(name, np.nan)
     assert np.array_equal(y[:, 1], np.full(3, low, NP[dt]), equal_nan=True)
+
+
+# ---- activations on their own: no sum, z is the bias ----
+
+def _grid():
+    z = np.r_[np.linspace(-13, 13, 4001), np.linspace(-0.5, 0.5, 2001), np.ldexp(1.0, np.arange(-120, 3)), -np.ldexp(1.0, np.arange(-120, 3))]
+    return z.astype(np.float32)
+
+
+def _exact(name, z):
+    """The activation in 64 bits, its small tail computed as a small number."""
+    z = z.astype(np.float64)
+    if name == "relu":
+        return np.maximum(z, 0.0)
+    if name == "gelu":
+        return 0.5 * z * np.vectorize(math.erfc)(-z / math.sqrt(2))
+    if name == "gelu_tanh":
+        return z / (1 + np.exp(-2 * math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3)))
+    if name == "silu":
+        return z / (1 + np.exp(-z))
+    return z
+
+
+def _units(name, z):
+    """How many 2^-24 of itself an activation may be off (thvm_hip.h): 8, and
+    what the rounding of an exponential's argument makes of it."""
+    z = np.abs(z.astype(np.float64))
+    return 8 + {"gelu": 2 * z * z, "gelu_tanh": 10 * (z + 0.045 * z ** 3), "silu": 2 * z}.get(name, 0.0)
+
+
+@pytest.mark.parametrize("name", ACTS)
+@pytest.mark.parametrize("dt", [F32, F16], ids=["f32", "f16"])
+def test_activation(hip, name, dt):
+    z = _grid().astype(NP[dt])
+    y, _ = bo.run_linear(hip, np.zeros((1, 0), NP[dt]), np.zeros((0, len(z)), NP[dt]), z, None, name, dt)
+    want = _exact(name, z)
+    within(y[0], want, _units(name, z) * U32 * np.abs(want) + bo.rounding(dt, want) + 2.0 ** -120)
+
+
+@pytest.mark.parametrize("name", ACTS[1:])
+def test_slope(hip, name):
+    """act' alone: the products of dy = 1 and its one partner 1 pass it on. Of
+    values around 0 and of far ones, within 16 (1 + |z|) units of 2^-24 of 1."""
+    z = _grid()
+    z = z[z != 0]
+    m = len(z)
+    dx, _, _ = bo.run_linear_grad(hip, np.ones((m, 1), np.float32), z[:, None], None, np.ones((1, 1), np.float32), name, F32, (True, False, False))
+    want = bo.slope(name, z)
+    within(dx[:, 0], want, 16 * U32 * (1 + np.abs(z.astype(np.float64))) * np.maximum(np.abs(want), 2.0 ** -3) + 2.0 ** -120)

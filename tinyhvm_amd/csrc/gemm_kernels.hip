@@ -62,15 +62,20 @@ __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf
 #define GELU_U 1.5957691216057308f
 #define GELU_C 0.044715f
 
-// The normal distribution's integral up to z, by the rational approximation of
-// erfc in Abramowitz and Stegun, 7.1.26: within 7.5e-8, a third of the
-// instructions of erff. Taken on the side of the small tail, so that a tail is
-// a small number and not what is left of 1.
+// The normal distribution's integral up to z. Near 0 it is 1/2 and an odd
+// polynomial; further out the small tail exp(-z^2 / 2) t P(t), t = 1 / (1 + 0.4
+// |z|), or what that leaves of 1. Both polynomials are least largest relative
+// errors, fitted to erf and exp(z^2 / 2) erfc: 7e-10 up to 1, 8e-8 up to 15. So a
+// tail is as exact as a value near 1, but for the rounding of the exponential's
+// argument: within (8 + 2 z^2) 2^-24 of itself. Half the instructions of erfcf.
 __device__ __forceinline__ float normal_cdf(float z) {
-    const float x = fabsf(z) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * x);
-    const float p = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
-    const float tail = 0.5f * p * __expf(-x * x);
-    return z < 0.0f ? tail : 1.0f - tail;
+    const float x = fabsf(z), u = z * z, t = __builtin_amdgcn_rcpf(1.0f + 0.4f * x);
+    const float near = 0.5f + z * (0.39894229174f + u * (-0.066490359604f + u * (0.0099733229727f + u * (-0.0011863299878f +
+                                   u * (0.00011348637054f + u * -7.6542091847e-06f)))));
+    const float p = t * (0.15959578753f + t * (0.15909999609f + t * (0.13900230825f + t * (0.055540546775f + t * (0.10536319017f +
+                         t * (-0.18642802537f + t * 0.068121381104f))))));
+    const float tail = p * __builtin_amdgcn_exp2f(-0.72134752044f * u);
+    return x <= 1.0f ? near : z < 0.0f ? tail : 1.0f - tail;
 }
 
 __device__ __forceinline__ float act_of(u32 act, float z) {
