@@ -80,6 +80,7 @@ def _plans():
         L = C.CDLL(so)
     f32, u32 = C.c_float, C.c_uint32
     L.thvm_hip_layer_norm.argtypes = [u32] * 8 + [f32, u32]
+    L.thvm_hip_muon_step.argtypes = [C.POINTER(u32)] * 3 + [u32] * 3 + [f32] * 4 + [u32] * 3
     return L
 
 
@@ -104,3 +105,8 @@ def linear(m, k, n, dtype):
 
 def linear_grad(m, k, n, dtype):
     return names("thvm_hip_linear_grad", 1, 2, 3, 4, 5, 6, 7, 1, m, k, n, dtype)
+
+
+def muon_step(count, rows, cols, dtype):
+    ids = [(C.c_uint32 * count)(*range(i * count + 1, (i + 1) * count + 1)) for i in range(3)]
+    return names("thvm_hip_muon_step", *ids, count, rows, cols, 0.1, 1.0, 0.0, 0.9, 1, 5, dtype)
