@@ -200,8 +200,8 @@ int  thvm_hip_linear_grad(u32 dx, u32 dw, u32 db, u32 dy, u32 z, u32 x, u32 w, u
  *   `steps` times:  A = X X^T, X = 3.4445 X + (-4.7750 A + 2.0315 A A) X
  *   param = (1 - lr weight_decay) param - lr scale X
  * |u| the Frobenius norm; the products run on the shorter side (X is u^T
- * where rows > cols). After 5 steps X's singular values lie between 0.68 and
- * 1.21 but for those that were under 1e-3 of |u|. `scale` is the caller's
+ * where rows > cols). After 5 steps X's singular values lie between 0.67 and
+ * 1.21 but for those that were under 1.5e-3 of |u|. `scale` is the caller's
  * choice for the shape, such as sqrt(max(1, outputs / inputs)) of a layer:
  * sqrt(max(1, cols / rows)) of W as thvm_hip_linear takes it. Of DTYPE_F16, X,
  * A and -4.7750 A + 2.0315 A A are rounded to 16 bits between products. */
