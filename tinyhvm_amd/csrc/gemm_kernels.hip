@@ -19,7 +19,7 @@
 // 32-bit operands are two f16 planes: x 2^e = hi + lo, hi the nearest f16 and
 // lo the nearest f16 of what is left, with e such that the largest value of
 // the row (the products' sums never mix rows) lies in [2^14, 2^15). hi + lo
-// is x 2^e to 2^-23 of itself, or to 2^-25 where x 2^e is under 2^-2. Of the
+// is x 2^e to 2^-23 of itself, or to 2^-24 where x 2^e is under 2^-2. Of the
 // four products three are summed, hi hi + hi lo + lo hi; lo lo is at most 2^-22
 // of the product. All sums are 32 bits. So a 32-bit product costs three 16-bit
 // ones, where three bf16 planes cost six, and a sum is within (2 K + 8) 2^-24
@@ -34,13 +34,13 @@
 // act'(z), rounded to 16 bits as a network in 16 bits holds it: of 2048^3 its
 // products' error against 64 bits is 2.9e-4, that of dz in 32 bits 2.1e-4, most
 // of it the outputs' own rounding, and a second plane for dz would double the
-// products' time. Where a dz is past 16 bits, the sums that it goes into are
+// products' instructions (now 47 of the call's 60 us). Where a dz is past 16 bits, the sums that it goes into are
 // computed again, too; packing tells the products of a call that there is one.
 //
-// Large tiles: of 4096^3 in 16 bits as they lie 135 us, 1018 TFLOP/s (a library
+// Large tiles: of 4096^3 in 16 bits as they lie 138 us, 995 TFLOP/s (a library
 // product 1155 on the same card; packed ones alone 129 us), the matrix units
-// busy 55 % of the cycles with one read of LDS a product; in 32 bits 318 us,
-// 1297 TFLOP/s of 16-bit products, busy 73 %. Either way the card holds its clock
+// busy 54 % of the cycles with one read of LDS a product; in 32 bits 324 us,
+// 1272 TFLOP/s of 16-bit products, busy 73 %. Either way the card holds its clock
 // near 1.7 GHz. Small ones are bound by the latency of one stage after another.
 #include <hip/hip_runtime.h>
 #include "thvm_abi.h"
