@@ -204,7 +204,8 @@ int  thvm_hip_linear_grad(u32 dx, u32 dw, u32 db, u32 dy, u32 z, u32 x, u32 w, u
  * 1.21 but for those that were under 1.5e-3 of |u|. `scale` is the caller's
  * choice for the shape, such as sqrt(max(1, outputs / inputs)) of a layer:
  * sqrt(max(1, cols / rows)) of W as thvm_hip_linear takes it. Of DTYPE_F16, X,
- * A and -4.7750 A + 2.0315 A A are rounded to 16 bits between products. */
+ * A and -4.7750 A + 2.0315 A A are rounded to 16 bits between products; of
+ * DTYPE_F32 they are held to 2^-23 of themselves, or to 2^-38. */
 int  thvm_hip_muon_step(const u32 *param, const u32 *grad, const u32 *m, u32 count, u32 rows, u32 cols, f32 lr, f32 scale,
                         f32 weight_decay, f32 beta, u32 nesterov, u32 steps, u32 dtype);
 
